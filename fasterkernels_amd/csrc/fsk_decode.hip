@@ -39,6 +39,7 @@
 #include <math.h>
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <string.h>
 #include <mutex>
 #include <string>
@@ -3639,6 +3640,8 @@ int run_write(const WriteArgs& a) {
   return FSK_OK;
 }
 
+#include "fsk_rope.h"
+
 template <int kSrc>
 void launch_quant(const QuantParams& p, unsigned grid, hipStream_t stream) {
   const Launch l{stream, nullptr, nullptr};
@@ -4313,6 +4316,60 @@ int fsk_paged_write(const void* k_new, int64_t k_stride_t, int64_t k_stride_h, c
   a.bt = block_table; a.bt_numel = bt_numel; a.upd = bt_updates; a.n_upd = num_bt_updates;
   a.stream = (hipStream_t)stream;
   return run_write(a);
+}
+
+int fsk_qk_norm_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                     int64_t k_stride_h, int64_t num_tokens, const void* cos, int64_t cos_stride, const void* sin,
+                     int64_t sin_stride, int64_t table_rows, int table_dtype, int rotary_dim, int interleaved,
+                     const int64_t* positions, const void* q_weight, const void* k_weight, int weight_dtype, float eps,
+                     void* q_out, int64_t qo_stride_t, int64_t qo_stride_h, void* k_out, int64_t ko_stride_t,
+                     int64_t ko_stride_h, int num_q_heads, int num_kv_heads, int head_dim, int dtype, void* stream) {
+  if (num_q_heads <= 0) return fail(FSK_ERR_INVALID, "heads and head_dim must be positive");
+  RopeArgs a;
+  memset(&a, 0, sizeof(a));
+  a.src[0] = q; a.s_st[0] = q_stride_t; a.s_sh[0] = q_stride_h;
+  a.src[1] = k; a.s_st[1] = k_stride_t; a.s_sh[1] = k_stride_h;
+  a.n = num_tokens;
+  a.cos = cos; a.c_sr = cos_stride; a.sin = sin; a.n_sr = sin_stride; a.t_rows = table_rows; a.t_dt = table_dtype;
+  a.rotary = rotary_dim; a.interleaved = interleaved; a.positions = positions;
+  a.weight[0] = q_weight; a.weight[1] = k_weight; a.w_dt = weight_dtype; a.eps = eps;
+  a.out[0] = q_out; a.o_st[0] = qo_stride_t; a.o_sh[0] = qo_stride_h;
+  a.out[1] = k_out; a.o_st[1] = ko_stride_t; a.o_sh[1] = ko_stride_h;
+  a.Hq = num_q_heads; a.Hkv = num_kv_heads; a.D = head_dim; a.src_dt = dtype;
+  a.stream = (hipStream_t)stream;
+  return run_rope(a);
+}
+
+int fsk_paged_write_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                         int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                         const int64_t* slot_mapping, int64_t num_tokens, const void* cos, int64_t cos_stride,
+                         const void* sin, int64_t sin_stride, int64_t table_rows, int table_dtype, int rotary_dim,
+                         int interleaved, const int64_t* positions, const void* q_weight, const void* k_weight,
+                         int weight_dtype, float eps, void* q_out, int64_t qo_stride_t, int64_t qo_stride_h,
+                         void* k_pool, int64_t k_stride_p, int64_t kp_stride_h, int64_t kp_stride_t, void* v_pool,
+                         int64_t v_stride_p, int64_t vp_stride_h, int64_t vp_stride_t, int num_pages, int page_size,
+                         int num_q_heads, int num_kv_heads, int head_dim, int src_dtype, int pool_dtype,
+                         const float* k_scale, const float* v_scale, int32_t* block_table, int64_t bt_numel,
+                         const int64_t* bt_updates, int64_t num_bt_updates, void* stream) {
+  RopeArgs a;
+  memset(&a, 0, sizeof(a));
+  a.src[0] = q; a.s_st[0] = q_stride_t; a.s_sh[0] = q_stride_h;
+  a.src[1] = k; a.s_st[1] = k_stride_t; a.s_sh[1] = k_stride_h;
+  a.src[2] = v; a.s_st[2] = v_stride_t; a.s_sh[2] = v_stride_h;
+  a.n = num_tokens; a.slots = slot_mapping;
+  a.cos = cos; a.c_sr = cos_stride; a.sin = sin; a.n_sr = sin_stride; a.t_rows = table_rows; a.t_dt = table_dtype;
+  a.rotary = rotary_dim; a.interleaved = interleaved; a.positions = positions;
+  a.weight[0] = q_weight; a.weight[1] = k_weight; a.w_dt = weight_dtype; a.eps = eps;
+  a.out[0] = q_out; a.o_st[0] = qo_stride_t; a.o_sh[0] = qo_stride_h;
+  a.paged = true;
+  a.pool[0] = k_pool; a.p_sp[0] = k_stride_p; a.p_sh[0] = kp_stride_h; a.p_st[0] = kp_stride_t;
+  a.pool[1] = v_pool; a.p_sp[1] = v_stride_p; a.p_sh[1] = vp_stride_h; a.p_st[1] = vp_stride_t;
+  a.num_pages = num_pages; a.page_size = page_size; a.Hq = num_q_heads; a.Hkv = num_kv_heads; a.D = head_dim;
+  a.src_dt = src_dtype; a.pool_dt = pool_dtype;
+  a.scale[0] = k_scale; a.scale[1] = v_scale;
+  a.bt = block_table; a.bt_numel = bt_numel; a.upd = bt_updates; a.n_upd = num_bt_updates;
+  a.stream = (hipStream_t)stream;
+  return run_rope(a);
 }
 
 }  // extern "C"

@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 #include <utility>
 #include <vector>
@@ -368,10 +369,8 @@ at::Tensor new_rows(const at::Tensor& t_in, const char* name) {
   return rows16(t);
 }
 
-void kv_write(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& k_pool, const at::Tensor& v_pool,
-           const at::Tensor& slot_mapping, const c10::optional<at::Tensor>& k_scale,
-           const c10::optional<at::Tensor>& v_scale, const c10::optional<at::Tensor>& block_table,
-           const c10::optional<at::Tensor>& bt_updates, int64_t stream) {
+// Pools of one layer, checked; with a contiguous head_dim.
+void check_pools(const at::Tensor& k_pool, const at::Tensor& v_pool) {
   for (const auto* pt : {&k_pool, &v_pool}) {
     const char* name = pt == &k_pool ? "k_pool" : "v_pool";
     on_gpu(*pt, name);
@@ -382,10 +381,57 @@ void kv_write(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& 
       raise(FSK_ERR_UNSUPPORTED, std::string(name) + ": dtype " + c10::toString(dt) + " (f16, bf16 or e4m3 expected)");
     if (pt->stride(-1) != 1) raise(FSK_ERR_INVALID, std::string(name) + " must have a contiguous head_dim");
   }
+  if (v_pool.device() != k_pool.device() || v_pool.sizes() != k_pool.sizes() ||
+      v_pool.scalar_type() != k_pool.scalar_type())
+    raise(FSK_ERR_INVALID, "k_pool and v_pool must match in shape, dtype and device");
+}
+
+at::Tensor slot_tensor(const at::Tensor& slot_mapping, int64_t n, const c10::Device& dev) {
+  on_device(slot_mapping, "slot_mapping", dev);
+  if (slot_mapping.scalar_type() != at::kLong || slot_mapping.numel() != n)
+    raise(FSK_ERR_INVALID, "slot_mapping must be int64 with " + std::to_string(n) + " entries");
+  return slot_mapping.dim() == 1 && slot_mapping.is_contiguous() ? slot_mapping : slot_mapping.reshape({n}).contiguous();
+}
+
+void check_write_scale(const c10::optional<at::Tensor>& s, const char* name, const c10::Device& dev) {
+  if (!s || !s->defined()) return;
+  if (s->scalar_type() != at::kFloat || s->numel() != 1)
+    raise(FSK_ERR_INVALID, std::string(name) + " must be a one-element fp32 device tensor");
+  on_device(*s, name, dev);
+}
+
+// Block-table stores of a write call.
+struct TableUpdates {
+  int32_t* table = nullptr;
+  int64_t numel = 0, n = 0;
+  at::Tensor upd;
+  const int64_t* data() const { return n ? upd.data_ptr<int64_t>() : nullptr; }
+};
+TableUpdates table_updates(const c10::optional<at::Tensor>& block_table, const c10::optional<at::Tensor>& bt_updates,
+                           const c10::Device& dev) {
+  TableUpdates u;
+  if (!bt_updates || !bt_updates->defined() || !bt_updates->numel()) return u;
+  if (!block_table || !block_table->defined()) raise(FSK_ERR_INVALID, "bt_updates need block_table");
+  on_device(*block_table, "block_table", dev);
+  on_device(*bt_updates, "bt_updates", dev);
+  if (block_table->scalar_type() != at::kInt || !block_table->is_contiguous())
+    raise(FSK_ERR_INVALID, "block_table must be a contiguous int32 tensor");
+  if (bt_updates->scalar_type() != at::kLong || bt_updates->dim() != 2 || bt_updates->size(1) != 2)
+    raise(FSK_ERR_INVALID, "bt_updates must be int64 [m, 2]");
+  u.upd = bt_updates->contiguous();
+  u.table = block_table->data_ptr<int32_t>();
+  u.numel = block_table->numel();
+  u.n = u.upd.size(0);
+  return u;
+}
+
+void kv_write(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& k_pool, const at::Tensor& v_pool,
+           const at::Tensor& slot_mapping, const c10::optional<at::Tensor>& k_scale,
+           const c10::optional<at::Tensor>& v_scale, const c10::optional<at::Tensor>& block_table,
+           const c10::optional<at::Tensor>& bt_updates, int64_t stream) {
+  check_pools(k_pool, v_pool);
   const c10::Device dev = k_pool.device();
   const c10::DeviceGuard guard(dev);
-  if (v_pool.device() != dev || v_pool.sizes() != k_pool.sizes() || v_pool.scalar_type() != k_pool.scalar_type())
-    raise(FSK_ERR_INVALID, "k_pool and v_pool must match in shape, dtype and device");
   const int64_t P = k_pool.size(0), Hkv = k_pool.size(1), PS = k_pool.size(2), D = k_pool.size(3);
   const at::Tensor k = new_rows(k_in, "k"), v = new_rows(v_in, "v");
   on_device(k, "k", dev);
@@ -394,43 +440,165 @@ void kv_write(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& 
   if (k.size(1) != Hkv || k.size(2) != D || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type())
     raise(FSK_ERR_INVALID, "k/v must be [" + std::to_string(n) + ", " + std::to_string(Hkv) + ", " +
                                std::to_string(D) + "] of one dtype, got " + shape_str(k) + " / " + shape_str(v));
-  on_device(slot_mapping, "slot_mapping", dev);
-  if (slot_mapping.scalar_type() != at::kLong || slot_mapping.numel() != n)
-    raise(FSK_ERR_INVALID, "slot_mapping must be int64 with " + std::to_string(n) + " entries");
-  const at::Tensor slots =
-      slot_mapping.dim() == 1 && slot_mapping.is_contiguous() ? slot_mapping : slot_mapping.reshape({n}).contiguous();
-  for (const auto* s : {&k_scale, &v_scale}) {
-    if (*s && (*s)->defined()) {
-      const char* name = s == &k_scale ? "k_scale" : "v_scale";
-      if ((*s)->scalar_type() != at::kFloat || (*s)->numel() != 1)
-        raise(FSK_ERR_INVALID, std::string(name) + " must be a one-element fp32 device tensor");
-      on_device(**s, name, dev);
-    }
-  }
-  int32_t* bt_ptr = nullptr;
-  int64_t bt_numel = 0, n_upd = 0;
-  at::Tensor upd;
-  if (bt_updates && bt_updates->defined() && bt_updates->numel()) {
-    if (!block_table || !block_table->defined()) raise(FSK_ERR_INVALID, "bt_updates need block_table");
-    on_device(*block_table, "block_table", dev);
-    on_device(*bt_updates, "bt_updates", dev);
-    if (block_table->scalar_type() != at::kInt || !block_table->is_contiguous())
-      raise(FSK_ERR_INVALID, "block_table must be a contiguous int32 tensor");
-    if (bt_updates->scalar_type() != at::kLong || bt_updates->dim() != 2 || bt_updates->size(1) != 2)
-      raise(FSK_ERR_INVALID, "bt_updates must be int64 [m, 2]");
-    upd = bt_updates->contiguous();
-    bt_ptr = block_table->data_ptr<int32_t>();
-    bt_numel = block_table->numel();
-    n_upd = upd.size(0);
-  }
+  const at::Tensor slots = slot_tensor(slot_mapping, n, dev);
+  check_write_scale(k_scale, "k_scale", dev);
+  check_write_scale(v_scale, "v_scale", dev);
+  const TableUpdates u = table_updates(block_table, bt_updates, dev);
   const int st = fsk_paged_write(
       k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr<int64_t>(), n,
       k_pool.data_ptr(), k_pool.stride(0), k_pool.stride(1), k_pool.stride(2), v_pool.data_ptr(), v_pool.stride(0),
       v_pool.stride(1), v_pool.stride(2), (int)P, (int)PS, (int)Hkv, (int)D, dtype_code(k.scalar_type(), "k"),
       dtype_code(k_pool.scalar_type(), "k_pool"), static_cast<const float*>(ptr_or_null(k_scale)),
-      static_cast<const float*>(ptr_or_null(v_scale)), bt_ptr, bt_numel,
-      n_upd ? upd.data_ptr<int64_t>() : nullptr, n_upd, stream_ptr(stream));
+      static_cast<const float*>(ptr_or_null(v_scale)), u.table, u.numel, u.data(), u.n, stream_ptr(stream));
   check(st);
+}
+
+// ---------------------------------------------------------------------------
+// Norm and rotation of query and key rows, to tensors or into the paged cache
+// ---------------------------------------------------------------------------
+// The kernels are not recorded: a call whose inputs want gradients is refused.
+void no_grad(std::initializer_list<const at::Tensor*> tensors, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : tensors)
+    if (t && t->defined() && t->requires_grad())
+      raise(kRuntime, std::string(what) + " has no backward pass: call it under torch.no_grad() or detach its inputs");
+}
+
+const at::Tensor* maybe(const c10::optional<at::Tensor>& t) { return t ? &*t : nullptr; }
+
+// A [n, H, D] tensor with rows the kernels can load, else a packed copy (an
+// unaligned contiguous tensor and a lazily negated one too).
+at::Tensor rope_rows(const at::Tensor& t, const char* name, const c10::Device& dev) {
+  on_device(t, name, dev);
+  if (t.dim() != 3) raise(FSK_ERR_INVALID, std::string(name) + " must be [n, heads, head_dim], got " + shape_str(t));
+  const auto dt = t.scalar_type();
+  if (dt != at::kHalf && dt != at::kBFloat16 && dt != at::kFloat)
+    raise(FSK_ERR_UNSUPPORTED, std::string(name) + ": dtype " + c10::toString(dt) + " (f16, bf16 or f32 expected)");
+  return has_rows16(t) && !t.is_neg() ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// cos and sin [rows, rotary_dim / 2], the positions and the norm weights.
+struct Rotation {
+  at::Tensor cos, sin, positions, qw, kw;
+  int64_t rows = 0, rotary = 0;
+  int t_dt = FSK_F32, w_dt = FSK_F32;
+};
+Rotation rotation(const c10::optional<at::Tensor>& cos, const c10::optional<at::Tensor>& sin,
+                  const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& q_weight,
+                  const c10::optional<at::Tensor>& k_weight, int64_t n, int64_t D, const c10::Device& dev) {
+  Rotation r;
+  auto given = [](const c10::optional<at::Tensor>& t) { return t && t->defined(); };
+  auto rows = [](const at::Tensor& t) { return has_rows16(t) && !t.is_neg() ? t : t.clone(at::MemoryFormat::Contiguous); };
+  if (given(cos) != given(sin)) raise(FSK_ERR_INVALID, "pass both cos and sin or neither");
+  if (given(cos)) {
+    on_device(*cos, "cos", dev);
+    on_device(*sin, "sin", dev);
+    if (cos->dim() != 2 || sin->sizes() != cos->sizes() || sin->scalar_type() != cos->scalar_type())
+      raise(FSK_ERR_INVALID, "cos and sin must be [rows, rotary_dim / 2] of one dtype, got " + shape_str(*cos) + " / " +
+                                 shape_str(*sin));
+    if (cos->size(1) < 1 || 2 * cos->size(1) > D)
+      raise(FSK_ERR_INVALID, "cos and sin hold " + std::to_string(cos->size(1)) + " pairs for a head_dim of " + std::to_string(D));
+    r.cos = rows(*cos);
+    r.sin = rows(*sin);
+    r.rows = r.cos.size(0);
+    r.rotary = 2 * r.cos.size(1);
+    r.t_dt = dtype_code(r.cos.scalar_type(), "cos");
+    if (given(positions)) {
+      on_device(*positions, "positions", dev);
+      const auto dt = positions->scalar_type();
+      if ((dt != at::kLong && dt != at::kInt) || positions->numel() != n)
+        raise(FSK_ERR_INVALID, "positions must be int64 or int32 with " + std::to_string(n) + " entries");
+      r.positions = positions->to(at::kLong).reshape({n}).contiguous();
+    }
+  } else if (given(positions)) {
+    raise(FSK_ERR_INVALID, "positions need cos and sin");
+  }
+  for (const auto* w : {&q_weight, &k_weight}) {
+    if (!given(*w)) continue;
+    const char* name = w == &q_weight ? "q_weight" : "k_weight";
+    on_device(**w, name, dev);
+    if ((*w)->dim() != 1 || (*w)->size(0) != D)
+      raise(FSK_ERR_INVALID, std::string(name) + " must hold head_dim=" + std::to_string(D) + " values, got " + shape_str(**w));
+    (w == &q_weight ? r.qw : r.kw) = rows(**w);
+    r.w_dt = dtype_code((*w)->scalar_type(), name);
+  }
+  if (r.qw.defined() && r.kw.defined() && r.qw.scalar_type() != r.kw.scalar_type())
+    raise(FSK_ERR_INVALID, "q_weight and k_weight must have one dtype");
+  return r;
+}
+const void* data_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+int64_t row_stride(const at::Tensor& t) { return t.defined() ? t.stride(0) : 0; }
+const int64_t* longs(const at::Tensor& t) { return t.defined() ? t.data_ptr<int64_t>() : nullptr; }
+
+std::pair<at::Tensor, at::Tensor> qk_norm_rope(
+    const at::Tensor& q_in, const at::Tensor& k_in, const c10::optional<at::Tensor>& cos,
+    const c10::optional<at::Tensor>& sin, const c10::optional<at::Tensor>& positions,
+    const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight, double eps, bool interleaved,
+    int64_t stream) {
+  on_gpu(q_in, "q");
+  const c10::Device dev = q_in.device();
+  const c10::DeviceGuard guard(dev);
+  no_grad({&q_in, &k_in, maybe(cos), maybe(sin), maybe(q_weight), maybe(k_weight)}, "qk_norm_rope");
+  const at::Tensor q = rope_rows(q_in, "q", dev), k = rope_rows(k_in, "k", dev);
+  const int64_t n = q.size(0), Hq = q.size(1), Hkv = k.size(1), D = q.size(2);
+  if (k.size(0) != n || k.size(2) != D || k.scalar_type() != q.scalar_type())
+    raise(FSK_ERR_INVALID, "q and k must be [n, heads, head_dim] of one dtype, got " + shape_str(q) + " / " + shape_str(k));
+  const Rotation r = rotation(cos, sin, positions, q_weight, k_weight, n, D, dev);
+  at::Tensor qo = at::empty({n, Hq, D}, q.options()), ko = at::empty({n, Hkv, D}, q.options());
+  check(fsk_qk_norm_rope(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), n,
+                         data_or_null(r.cos), row_stride(r.cos), data_or_null(r.sin), row_stride(r.sin), r.rows, r.t_dt,
+                         (int)r.rotary, interleaved, longs(r.positions), data_or_null(r.qw), data_or_null(r.kw), r.w_dt,
+                         (float)eps, qo.data_ptr(), qo.stride(0), qo.stride(1), ko.data_ptr(), ko.stride(0),
+                         ko.stride(1), (int)Hq, (int)Hkv, (int)D, dtype_code(q.scalar_type(), "q"), stream_ptr(stream)));
+  return {qo, ko};
+}
+
+c10::optional<at::Tensor> kv_write_rope(
+    const c10::optional<at::Tensor>& q_in, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& k_pool,
+    const at::Tensor& v_pool, const at::Tensor& slot_mapping, const c10::optional<at::Tensor>& cos,
+    const c10::optional<at::Tensor>& sin, const c10::optional<at::Tensor>& positions,
+    const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight, double eps, bool interleaved,
+    const c10::optional<at::Tensor>& k_scale, const c10::optional<at::Tensor>& v_scale,
+    const c10::optional<at::Tensor>& block_table, const c10::optional<at::Tensor>& bt_updates, int64_t stream) {
+  check_pools(k_pool, v_pool);
+  const c10::Device dev = k_pool.device();
+  const c10::DeviceGuard guard(dev);
+  no_grad({maybe(q_in), &k_in, &v_in, maybe(cos), maybe(sin), maybe(q_weight), maybe(k_weight)}, "paged_kv_write_rope");
+  const int64_t P = k_pool.size(0), Hkv = k_pool.size(1), PS = k_pool.size(2), D = k_pool.size(3);
+  const at::Tensor k = rope_rows(k_in, "k", dev), v = rope_rows(v_in, "v", dev);
+  const int64_t n = k.size(0);
+  if (k.size(1) != Hkv || k.size(2) != D || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type())
+    raise(FSK_ERR_INVALID, "k/v must be [" + std::to_string(n) + ", " + std::to_string(Hkv) + ", " +
+                               std::to_string(D) + "] of one dtype, got " + shape_str(k) + " / " + shape_str(v));
+  at::Tensor q, qo;
+  int64_t Hq = 0;
+  if (q_in && q_in->defined()) {
+    q = rope_rows(*q_in, "q", dev);
+    Hq = q.size(1);
+    if (q.size(0) != n || q.size(2) != D || q.scalar_type() != k.scalar_type() || Hq < 1)
+      raise(FSK_ERR_INVALID, "q must be [" + std::to_string(n) + ", heads, " + std::to_string(D) + "] of k's dtype, got " +
+                                 shape_str(q));
+    qo = at::empty({n, Hq, D}, q.options());
+  } else if (q_weight && q_weight->defined()) {
+    raise(FSK_ERR_INVALID, "q_weight without q");
+  }
+  const Rotation r = rotation(cos, sin, positions, q_weight, k_weight, n, D, dev);
+  const at::Tensor slots = slot_tensor(slot_mapping, n, dev);
+  check_write_scale(k_scale, "k_scale", dev);
+  check_write_scale(v_scale, "v_scale", dev);
+  const TableUpdates u = table_updates(block_table, bt_updates, dev);
+  check(fsk_paged_write_rope(
+      data_or_null(q), row_stride(q), Hq ? q.stride(1) : 0, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+      v.stride(0), v.stride(1), slots.data_ptr<int64_t>(), n, data_or_null(r.cos), row_stride(r.cos),
+      data_or_null(r.sin), row_stride(r.sin), r.rows, r.t_dt, (int)r.rotary, interleaved, longs(r.positions),
+      data_or_null(r.qw), data_or_null(r.kw), r.w_dt, (float)eps, Hq ? qo.data_ptr() : nullptr, row_stride(qo),
+      Hq ? qo.stride(1) : 0, k_pool.data_ptr(), k_pool.stride(0), k_pool.stride(1), k_pool.stride(2),
+      v_pool.data_ptr(), v_pool.stride(0), v_pool.stride(1), v_pool.stride(2), (int)P, (int)PS, (int)Hq, (int)Hkv,
+      (int)D, dtype_code(k.scalar_type(), "k"), dtype_code(k_pool.scalar_type(), "k_pool"),
+      static_cast<const float*>(ptr_or_null(k_scale)), static_cast<const float*>(ptr_or_null(v_scale)), u.table,
+      u.numel, u.data(), u.n, stream_ptr(stream)));
+  if (!Hq) return c10::nullopt;
+  return qo;
 }
 
 // ---------------------------------------------------------------------------
@@ -639,4 +807,10 @@ PYBIND11_MODULE(_fsk_torch, m) {
   m.def("quantize", &quantize, py::arg("tensors"), py::arg("stream"));
   m.def("kv_write", &kv_write, py::arg("k"), py::arg("v"), py::arg("k_pool"), py::arg("v_pool"), py::arg("slot_mapping"),
         py::arg("k_scale"), py::arg("v_scale"), py::arg("block_table"), py::arg("bt_updates"), py::arg("stream"));
+  m.def("qk_norm_rope", &qk_norm_rope, py::arg("q"), py::arg("k"), py::arg("cos"), py::arg("sin"), py::arg("positions"),
+        py::arg("q_weight"), py::arg("k_weight"), py::arg("eps"), py::arg("interleaved"), py::arg("stream"));
+  m.def("kv_write_rope", &kv_write_rope, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("k_pool"), py::arg("v_pool"),
+        py::arg("slot_mapping"), py::arg("cos"), py::arg("sin"), py::arg("positions"), py::arg("q_weight"),
+        py::arg("k_weight"), py::arg("eps"), py::arg("interleaved"), py::arg("k_scale"), py::arg("v_scale"),
+        py::arg("block_table"), py::arg("bt_updates"), py::arg("stream"));
 }

@@ -304,6 +304,54 @@ FSK_API int fsk_paged_write(const void *k_new, int64_t k_stride_t, int64_t k_str
                     const int64_t *bt_updates, int64_t num_bt_updates,
                     void *stream);
 
+/* Per-head RMS norm and position rotation of a batch of tokens' query and key
+ * rows, in one pass and one launch.  No counterpart in the reference (its
+ * models run them as torch operations in front of the attention function).
+ * q [n, Hq, D] and k [n, Hkv, D] (token stride, head stride; head_dim
+ * contiguous, 16-byte aligned rows, D a multiple of 16 up to 256) in f16, bf16
+ * or f32; outputs of the same type, which may be the inputs themselves.  Per
+ * head row x at position p:
+ *   y = x / sqrt(mean(x^2) + eps) * weight       (no norm where the weight is NULL)
+ *   (y_i, y_j) = (y_i cos - y_j sin, y_j cos + y_i sin), cos = cos[p][t],
+ * for t < rotary_dim / 2 and (i, j) = (t, t + rotary_dim / 2), or (2t, 2t + 1)
+ * when `interleaved`; other dims keep y.  fp32 throughout, rounded once.
+ * cos / sin [table_rows, rotary_dim / 2] (row strides, 16-byte aligned rows) in
+ * f16, bf16 or f32, shared by all heads; rotary_dim a multiple of 16 (0: norm
+ * only, tables unused).  positions int64 [n] (device; values outside the table
+ * take its first or last row), or NULL: token i takes row i mod table_rows, and
+ * table_rows divides n. */
+FSK_API int fsk_qk_norm_rope(const void *q, int64_t q_stride_t, int64_t q_stride_h,
+                     const void *k, int64_t k_stride_t, int64_t k_stride_h, int64_t num_tokens,
+                     const void *cos, int64_t cos_stride, const void *sin, int64_t sin_stride,
+                     int64_t table_rows, int table_dtype, int rotary_dim, int interleaved,
+                     const int64_t *positions,
+                     const void *q_weight, const void *k_weight, int weight_dtype, float eps,
+                     void *q_out, int64_t qo_stride_t, int64_t qo_stride_h,
+                     void *k_out, int64_t ko_stride_t, int64_t ko_stride_h,
+                     int num_q_heads, int num_kv_heads, int head_dim, int dtype, void *stream);
+
+/* fsk_paged_write with the norm and rotation of fsk_qk_norm_rope applied to the
+ * keys on the way into the pool (rounded once, to the pool's type; e4m3 pools
+ * with scales store e4m3(clamp(y / scale, +-448))) and to the queries, which go
+ * to q_out in src_dtype (num_q_heads = 0: no queries).  Values, slots, scales
+ * and block-table updates as fsk_paged_write takes them; a token whose slot is
+ * out of range keeps its queries.  Tokens that share a slot race. */
+FSK_API int fsk_paged_write_rope(const void *q, int64_t q_stride_t, int64_t q_stride_h,
+                     const void *k, int64_t k_stride_t, int64_t k_stride_h,
+                     const void *v, int64_t v_stride_t, int64_t v_stride_h,
+                     const int64_t *slot_mapping, int64_t num_tokens,
+                     const void *cos, int64_t cos_stride, const void *sin, int64_t sin_stride,
+                     int64_t table_rows, int table_dtype, int rotary_dim, int interleaved,
+                     const int64_t *positions,
+                     const void *q_weight, const void *k_weight, int weight_dtype, float eps,
+                     void *q_out, int64_t qo_stride_t, int64_t qo_stride_h,
+                     void *k_pool, int64_t k_stride_p, int64_t k_stride_h_pool, int64_t k_stride_t_pool,
+                     void *v_pool, int64_t v_stride_p, int64_t v_stride_h_pool, int64_t v_stride_t_pool,
+                     int num_pages, int page_size, int num_q_heads, int num_kv_heads, int head_dim,
+                     int src_dtype, int pool_dtype, const float *k_scale, const float *v_scale,
+                     int32_t *block_table, int64_t bt_numel,
+                     const int64_t *bt_updates, int64_t num_bt_updates, void *stream);
+
 /* Debug: gather a paged pool into a dense [B, Hkv, max_blocks*page_size, D]
  * tensor through the decode kernels' own page-addressing routine; rows at or
  * past seq_lens[b] are written as zero.  Bit-exact copy of the element bytes.
