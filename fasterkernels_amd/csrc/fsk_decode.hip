@@ -43,6 +43,7 @@
 #include <string.h>
 #include <mutex>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 #include "fsk_decode.h"
@@ -1689,12 +1690,18 @@ struct ReduceParams {
   const int32_t* lens;
   uint8_t* scores;     // [B, Hq, nblk] in the output dtype, contiguous
   int nblk;
+  // Shared prefix (kShared kernels only): partials [n_pre, Hkv, B G] of every
+  // sequence's rows over the shared tokens.
+  const float* pre_ml;
+  const float* pre_acc;
+  int n_pre;
+  int pre_rows;        // B G
 };
 
 constexpr int kReduceThreads = 256;
 
 // Rows h0 .. h0 + kRows - 1 (query heads) of sequence b (tid: threadIdx.x).
-template <int D, int kOut, int kRows>
+template <int D, int kOut, int kRows, bool kShared>
 __device__ __forceinline__ void reduce_rows(const ReduceParams& p, int h0, int b, int tid) {
   // Thread t of row r = t / (256 / kRows) owns the float4 column d4 = t %
   // (D/4) of unit group grp; group grp merges units grp, grp + kGroups, ...
@@ -1722,6 +1729,10 @@ __device__ __forceinline__ void reduce_rows(const ReduceParams& p, int h0, int b
   const int n = p.plan[b + 1] - u0;
   const int64_t base = ((int64_t)u0 * p.Hkv + kvh) * p.G + hg;  // partial index of unit u0
   const int64_t ustride = (int64_t)p.Hkv * p.G;                 // between consecutive units
+  // with a shared prefix its partials follow the sequence's own
+  const int n_all = kShared ? n + p.n_pre : n;
+  const int64_t pre_base = kShared ? (int64_t)kvh * p.pre_rows + (int64_t)b * p.G + hg : 0;
+  const int64_t pre_stride = kShared ? (int64_t)p.Hkv * p.pre_rows : 0;
   // Block scores: every thread loads up to kScorePre of this row's block
   // maxima now, in the same round trip as the partials, and stores their
   // scores once the denominator is known.
@@ -1738,13 +1749,17 @@ __device__ __forceinline__ void reduce_rows(const ReduceParams& p, int h0, int b
 
   float m_t = -INFINITY, l_t = 0.f;
   f32x4 a_t = {0.f, 0.f, 0.f, 0.f};
-  for (int i0 = grp; i0 < n; i0 += kGroups * kPer) {
+  for (int i0 = grp; i0 < n_all; i0 += kGroups * kPer) {
     f32x2 ml[kPer];
     f32x4 ac[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int i = i0 + j * kGroups;
-      if (i < n) {
+      if (kShared && i >= n && i < n_all) {
+        const int64_t idx = pre_base + (i - n) * pre_stride;
+        ml[j] = *(const f32x2*)(p.pre_ml + 2 * idx);
+        ac[j] = *(const f32x4*)(p.pre_acc + idx * D + 4 * d4);
+      } else if (i < n) {
         const int64_t idx = base + i * ustride;
         ml[j] = *(const f32x2*)(p.part_ml + 2 * idx);
         ac[j] = *(const f32x4*)(p.part_acc + idx * D + 4 * d4);
@@ -1827,9 +1842,9 @@ __device__ __forceinline__ void reduce_rows(const ReduceParams& p, int h0, int b
 }
 
 // One workgroup per (query head, sequence).
-template <int D, int kOut>
+template <int D, int kOut, bool kShared>
 __global__ __launch_bounds__(kReduceThreads) void reduce_kernel(ReduceParams p) {
-  reduce_rows<D, kOut, 1>(p, blockIdx.x, blockIdx.y, threadIdx.x);
+  reduce_rows<D, kOut, 1, kShared>(p, blockIdx.x, blockIdx.y, threadIdx.x);
 }
 
 // For many rows (more than the 2048 workgroups that fit the chip at once),
@@ -1852,13 +1867,13 @@ __global__ __launch_bounds__(kReduceThreads) void reduce_kernel(ReduceParams p) 
 // wide table: 32.1, with 256 29.2, with 128 29.0).
 constexpr int kFewUnits = 16;    // partials of a sequence that count as few
 constexpr int kLongGroups = 256;
-template <int D, int kOut, int kManyRows>
+template <int D, int kOut, int kManyRows, bool kShared>
 __global__ __launch_bounds__(kReduceThreads) void reduce_many_kernel(ReduceParams p, int B, FastDiv per_seq) {
   if ((int)blockIdx.x >= kLongGroups) {
     const uint32_t i = blockIdx.x - kLongGroups;
     const uint32_t b = fdiv(i, per_seq);  // per_seq = Hq / kManyRows workgroups of a sequence
     if (p.plan[b + 1] - p.plan[b] > kFewUnits) return;
-    reduce_rows<D, kOut, kManyRows>(p, (int)(i - b * per_seq.d) * kManyRows, (int)b, threadIdx.x);
+    reduce_rows<D, kOut, kManyRows, kShared>(p, (int)(i - b * per_seq.d) * kManyRows, (int)b, threadIdx.x);
     return;
   }
   constexpr int kPasses = 4;  // of kReduceThreads sequences, in one round trip
@@ -1896,7 +1911,7 @@ __global__ __launch_bounds__(kReduceThreads) void reduce_many_kernel(ReduceParam
       // it took 94 registers, with which five workgroups fit a CU, not seven)
       int tid = threadIdx.x;
       asm volatile("" : "+v"(tid));
-      reduce_rows<D, kOut, 1>(p, row - k * p.Hq, seq, tid);
+      reduce_rows<D, kOut, 1, kShared>(p, row - k * p.Hq, seq, tid);
       __syncthreads();
     }
     before += here;
@@ -2983,6 +2998,8 @@ struct Common {
   bool no_timing;          // never stamp this call (no event creation: the allocation-free entry)
   const struct QuantPre* pre;  // quantising decode (dense, f16 / bf16): its first launch, or null
   bool lens_on_host;       // lens is host memory: the plan is built here (make_host_plan)
+  const struct SharedParts* shared;  // partials of a shared prefix that the reduce takes in, or null
+  hipEvent_t last;         // stamped by the last launch (a shared decode's timed call), or null
 };
 
 bool aligned(const void* p, int a) { return ((uintptr_t)p % a) == 0; }
@@ -3147,21 +3164,21 @@ FastDiv make_fastdiv(uint32_t d) {
   return FastDiv{d, (uint32_t)((two_s + d - 1) / d), 31 + l};
 }
 
-template <int D, int kOut>
+template <int D, int kOut, bool kShared>
 void launch_reduce_out(const ReduceParams& rp, int B, int rows, const Launch& s) {
   if (rows == 1) {
-    launch(reduce_kernel<D, kOut>, dim3(rp.Hq, B), dim3(kReduceThreads), 0, s, rp);
+    launch(reduce_kernel<D, kOut, kShared>, dim3(rp.Hq, B), dim3(kReduceThreads), 0, s, rp);
     return;
   }
   const dim3 grid((unsigned)(kLongGroups + (int64_t)rp.Hq / rows * B));
   const FastDiv per_seq = make_fastdiv((uint32_t)(rp.Hq / rows));
   if constexpr (D <= 128) {
     if (rows == 8) {
-      launch(reduce_many_kernel<D, kOut, 8>, grid, dim3(kReduceThreads), 0, s, rp, B, per_seq);
+      launch(reduce_many_kernel<D, kOut, 8, kShared>, grid, dim3(kReduceThreads), 0, s, rp, B, per_seq);
       return;
     }
   }
-  launch(reduce_many_kernel<D, kOut, 4>, grid, dim3(kReduceThreads), 0, s, rp, B, per_seq);
+  launch(reduce_many_kernel<D, kOut, 4, kShared>, grid, dim3(kReduceThreads), 0, s, rp, B, per_seq);
 }
 
 // More rows than workgroups fit at once (2048 of 256 threads on 256 CUs): see
@@ -3175,9 +3192,14 @@ void launch_reduce(const ReduceParams& rp, int B, int o_dt, const Launch& s) {
   const int64_t total = (int64_t)rp.Hq * B;
   int rows = D <= 128 && rp.Hq % 8 == 0 ? 8 : rp.Hq % 4 == 0 ? 4 : 1;
   if (total <= 2048 || total / rows + kLongGroups >= (1 << 24) || rp.scores) rows = 1;
-  if (o_dt == FSK_F16) launch_reduce_out<D, kF16>(rp, B, rows, s);
-  else if (o_dt == FSK_BF16) launch_reduce_out<D, kBF16>(rp, B, rows, s);
-  else launch_reduce_out<D, kF32>(rp, B, rows, s);
+  auto out = [&](auto shared) {
+    constexpr bool kShared = decltype(shared)::value;
+    if (o_dt == FSK_F16) launch_reduce_out<D, kF16, kShared>(rp, B, rows, s);
+    else if (o_dt == FSK_BF16) launch_reduce_out<D, kBF16, kShared>(rp, B, rows, s);
+    else launch_reduce_out<D, kF32, kShared>(rp, B, rows, s);
+  };
+  if (rp.n_pre > 0) out(std::true_type{});
+  else out(std::false_type{});
 }
 
 // The split policy's per-call constants (see SplitArgs): target_units <=
@@ -3378,6 +3400,8 @@ int direct_waves(const Common& c, int64_t groups, bool pair) {
   return waves;
 }
 
+#include "fsk_prefix.h"
+
 int run_decode(const Common& c) {
   int st = validate(c);
   if (st != FSK_OK) return st;
@@ -3467,7 +3491,7 @@ int run_decode(const Common& c) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(FSK_ERR_HIP, std::string("range and maxima kernel launch failed: ") + hipGetErrorString(e));
   }
-  if (const int waves = direct_waves(c, (int64_t)c.B * p.n_items_h, pair)) {
+  if (const int waves = c.shared ? 0 : direct_waves(c, (int64_t)c.B * p.n_items_h, pair)) {
     DirectParams dp;
     memset(&dp, 0, sizeof(dp));
     dp.p = p;
@@ -3530,12 +3554,17 @@ int run_decode(const Common& c) {
   }
 
   ReduceParams rp;
+  memset(&rp, 0, sizeof(rp));
+  if (c.shared) {
+    rp.pre_ml = c.shared->ml; rp.pre_acc = c.shared->acc; rp.n_pre = c.shared->n;
+    rp.pre_rows = c.B * G;
+  }
   rp.plan = p.plan; rp.part_ml = p.part_ml; rp.part_acc = p.part_acc;
   rp.s_aux = c.s_aux; rp.sink_mode = c.sink_mode;
   rp.out = (uint8_t*)c.out; rp.o_sb = c.o_sb * oe; rp.o_sh = c.o_sh * oe;
   rp.Hq = c.Hq; rp.Hkv = c.Hkv; rp.G = G;
   rp.blk_max = p.blk_max; rp.lens = p.lens_out; rp.scores = (uint8_t*)c.scores; rp.nblk = c.nblk;
-  const Launch lr{c.stream, nullptr, ev[2]};
+  const Launch lr{c.stream, nullptr, c.last ? c.last : ev[2]};
   if (c.D == 64) launch_reduce<64>(rp, c.B, c.o_dt, lr);
   else if (c.D == 128) launch_reduce<128>(rp, c.B, c.o_dt, lr);
   else launch_reduce<256>(rp, c.B, c.o_dt, lr);
@@ -3543,6 +3572,107 @@ int run_decode(const Common& c) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(FSK_ERR_HIP, std::string("kernel launch failed: ") + hipGetErrorString(e));
   return FSK_OK;
+}
+
+// Workspace of a shared-prefix decode: the own lengths, the prefix's partials,
+// then the workspace of the decode of the own tokens.
+struct SharedLayout {
+  int64_t ml_off, acc_off, own_off;
+};
+SharedLayout shared_layout(const PrefixPlan& pl, int B, int Hq, int D) {
+  SharedLayout w;
+  w.ml_off = align256(4 * (int64_t)B);
+  w.acc_off = w.ml_off + align256((int64_t)pl.chunks * B * Hq * 2 * 4);
+  w.own_off = w.acc_off + align256((int64_t)pl.chunks * B * Hq * (int64_t)D * 4);
+  return w;
+}
+int64_t own_workspace(int B, int Hq, int Hkv, int D, int own_blocks, int page_size) {
+  return fsk_workspace_bytes(FSK_LAYOUT_PAGED, B, Hq, Hkv, D, own_blocks, page_size, 0);
+}
+int64_t shared_workspace(int B, int Hq, int Hkv, int D, int64_t max_blocks, int page_size, int64_t shared_len) {
+  const int64_t whole = fsk_workspace_bytes(FSK_LAYOUT_PAGED, B, Hq, Hkv, D, max_blocks, page_size, 0);
+  if (whole < 0) return whole;
+  if (shared_len < 0 || shared_len > max_blocks * page_size)
+    return fail(FSK_ERR_INVALID, "shared_len must be in [0, max_blocks * page_size]");
+  const int64_t common = shared_len / page_size;
+  if (common == 0 || B == 0) return whole;
+  const PrefixPlan pl = plan_prefix((int64_t)B * (Hq / Hkv), Hkv, D, common * page_size, device_cus());
+  const int64_t own = own_workspace(B, Hq, Hkv, D, (int)(max_blocks - common), page_size);
+  if (own < 0) return own;
+  return shared_layout(pl, B, Hq, D).own_off + own;
+}
+
+// Paged decode whose sequences share their first shared_len tokens' pages:
+// prefix_kernel over the shared pages, the split kernel over each sequence's
+// own (its lengths come from the prefix kernel), and the reduce over both.
+int run_shared(const Common& c, int64_t shared_len) {
+  int st = validate(c);
+  if (st != FSK_OK) return st;
+  if (shared_len < 0 || shared_len > (int64_t)c.max_blocks * c.page_size)
+    return fail(FSK_ERR_INVALID, "shared_len must be in [0, max_blocks * page_size]");
+  const int common = (int)(shared_len / c.page_size);  // whole shared pages
+  if (c.B == 0 || common == 0) return run_decode(c);
+  const int G = c.Hq / c.Hkv;
+  const PrefixPlan pl = plan_prefix((int64_t)c.B * G, c.Hkv, c.D, (int64_t)common * c.page_size, device_cus());
+  const int64_t grid = cdiv((int64_t)pl.chunks * c.Hkv, 8) * 8 * pl.row_tiles;
+  if (grid >= (1 << 24)) return fail(FSK_ERR_UNSUPPORTED, "too many work units");
+  const SharedLayout wl = shared_layout(pl, c.B, c.Hq, c.D);
+  const int64_t own_ws = own_workspace(c.B, c.Hq, c.Hkv, c.D, c.max_blocks - common, c.page_size);
+  if (own_ws < 0) return (int)own_ws;
+  if (!c.ws || c.ws_bytes < wl.own_off + own_ws || !aligned(c.ws, 256))
+    return fail(FSK_ERR_WORKSPACE, "workspace missing, unaligned or smaller than fsk_shared_workspace_bytes()");
+  uint8_t* ws = (uint8_t*)c.ws;
+  const SharedParts parts{(float*)(ws + wl.ml_off), (float*)(ws + wl.acc_off), pl.chunks};
+  Common own = c;
+  own.bt = c.bt + common;
+  own.max_blocks = c.max_blocks - common;
+  own.kv_extent = own.max_blocks;
+  own.lens = (const int32_t*)ws;
+  own.ws = ws + wl.own_off;
+  own.ws_bytes = c.ws_bytes - wl.own_off;
+  own.shared = &parts;
+  own.no_timing = true;
+
+  const int qe = elem_bytes(c.q_dt), ke = elem_bytes(c.kv_dt);
+  PrefixParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = (const uint8_t*)c.q;
+  p.q_sb = c.q_sb * qe; p.q_sh = c.q_sh * qe;
+  p.k = (const uint8_t*)c.k; p.v = (const uint8_t*)c.v;
+  p.k_sp = c.k_s0 * ke; p.k_sh = c.k_sh * ke; p.k_st = c.k_st * ke;
+  p.v_sp = c.v_s0 * ke; p.v_sh = c.v_sh * ke; p.v_st = c.v_st * ke;
+  p.pages = c.bt;
+  p.page = make_fastdiv((uint32_t)c.page_size);
+  p.num_pages = c.num_pages;
+  p.lens = c.lens; p.own_lens = (int32_t*)ws;
+  p.max_len = c.max_blocks * c.page_size;
+  p.k_scale = c.k_scale; p.v_scale = c.v_scale;
+  p.score_scale = c.sm_scale * kLog2e;
+  p.B = c.B; p.G = G; p.Hkv = c.Hkv; p.rows = c.B * G;
+  p.g_div = make_fastdiv((uint32_t)G);
+  p.hkv_div = make_fastdiv((uint32_t)c.Hkv);
+  p.rt_div = make_fastdiv((uint32_t)pl.row_tiles);
+  p.tokens = common * c.page_size; p.tiles = pl.tiles; p.chunk = pl.chunk;
+  p.units = pl.chunks * c.Hkv;
+  p.part_ml = (float*)(ws + wl.ml_off); p.part_acc = (float*)(ws + wl.acc_off);
+  (void)hipGetLastError();
+  // Timed calls: the prefix kernel's dispatch stamps its start and end, the
+  // last launch its end.
+  hipEvent_t ev[3] = {nullptr, nullptr, nullptr};
+  if (!c.no_timing) timing_events(ev);
+  const Launch l{c.stream, ev[0], ev[1]};
+  if (c.D == 64) launch_prefix<64>(p, c.q_dt, c.kv_dt, pl.waves, (unsigned)grid, l);
+  else if (c.D == 128) launch_prefix<128>(p, c.q_dt, c.kv_dt, pl.waves, (unsigned)grid, l);
+  else launch_prefix<256>(p, c.q_dt, c.kv_dt, pl.waves, (unsigned)grid, l);
+  const hipError_t e = hipGetLastError();  // (the decode below clears the error state before its launches)
+  if (e != hipSuccess) {
+    timing_keep(ev, false);
+    return fail(FSK_ERR_HIP, std::string("prefix kernel launch failed: ") + hipGetErrorString(e));
+  }
+  own.last = ev[2];
+  st = run_decode(own);
+  timing_keep(ev, st == FSK_OK);
+  return st;
 }
 
 
@@ -4316,6 +4446,35 @@ int fsk_paged_write(const void* k_new, int64_t k_stride_t, int64_t k_stride_h, c
   a.bt = block_table; a.bt_numel = bt_numel; a.upd = bt_updates; a.n_upd = num_bt_updates;
   a.stream = (hipStream_t)stream;
   return run_write(a);
+}
+
+int64_t fsk_shared_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim, int64_t max_blocks,
+                                   int page_size, int64_t shared_len) {
+  return shared_workspace(batch, num_q_heads, num_kv_heads, head_dim, max_blocks, page_size, shared_len);
+}
+
+int fsk_decode_paged_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_pool,
+                            int64_t k_stride_p, int64_t k_stride_h, int64_t k_stride_t, const void* v_pool,
+                            int64_t v_stride_p, int64_t v_stride_h, int64_t v_stride_t, const int32_t* block_table,
+                            int64_t bt_stride_b, int max_blocks, const int32_t* seq_lens, int64_t shared_len,
+                            int num_pages, int page_size, const float* s_aux, int sink_mode, const float* k_scale,
+                            const float* v_scale, void* out, int64_t o_stride_b, int64_t o_stride_h, int batch,
+                            int num_q_heads, int num_kv_heads, int head_dim, int q_dtype, int kv_dtype, int out_dtype,
+                            float sm_scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  Common c;
+  memset(&c, 0, sizeof(c));
+  c.layout = FSK_LAYOUT_PAGED;
+  c.q = q; c.q_sb = q_stride_b; c.q_sh = q_stride_h;
+  c.k = k_pool; c.k_s0 = k_stride_p; c.k_sh = k_stride_h; c.k_st = k_stride_t;
+  c.v = v_pool; c.v_s0 = v_stride_p; c.v_sh = v_stride_h; c.v_st = v_stride_t;
+  c.bt = block_table; c.bt_sb = bt_stride_b; c.max_blocks = max_blocks;
+  c.lens = seq_lens; c.num_pages = num_pages; c.page_size = page_size; c.kv_extent = max_blocks;
+  c.s_aux = s_aux; c.sink_mode = sink_mode; c.k_scale = k_scale; c.v_scale = v_scale;
+  c.out = out; c.o_sb = o_stride_b; c.o_sh = o_stride_h;
+  c.B = batch; c.Hq = num_q_heads; c.Hkv = num_kv_heads; c.D = head_dim;
+  c.q_dt = q_dtype; c.kv_dt = kv_dtype; c.o_dt = out_dtype; c.sm_scale = sm_scale;
+  c.ws = workspace; c.ws_bytes = workspace_bytes; c.stream = (hipStream_t)stream;
+  return run_shared(c, shared_len);
 }
 
 int fsk_qk_norm_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,

@@ -178,6 +178,14 @@ c10::DataPtr workspace(int64_t nbytes, const at::Tensor& out) {
   return allocator->allocate((size_t)nbytes);
 }
 
+// The kernels are not recorded: a call whose inputs want gradients is refused.
+void no_grad(std::initializer_list<const at::Tensor*> tensors, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : tensors)
+    if (t && t->defined() && t->requires_grad())
+      raise(kRuntime, std::string(what) + " has no backward pass: call it under torch.no_grad() or detach its inputs");
+}
+
 void* stream_ptr(int64_t stream) { return reinterpret_cast<void*>(static_cast<intptr_t>(stream)); }
 
 // ---------------------------------------------------------------------------
@@ -247,6 +255,51 @@ at::Tensor paged(const at::Tensor& q_in, const at::Tensor& k_pool, const at::Ten
                                  stream_ptr(stream));
   }
   check(st);
+  return out;
+}
+
+// ---------------------------------------------------------------------------
+// paged, with a prefix that all sequences share
+// ---------------------------------------------------------------------------
+at::Tensor paged_shared(const at::Tensor& q_in, const at::Tensor& k_pool, const at::Tensor& v_pool,
+                        const at::Tensor& block_table, const at::Tensor& seq_lens, int64_t page_size,
+                        int64_t shared_len, const c10::optional<at::Tensor>& s_aux,
+                        const c10::optional<at::Tensor>& k_scale, const c10::optional<at::Tensor>& v_scale,
+                        int64_t out_code, int64_t sink_mode, c10::optional<double> sm_scale, int64_t stream) {
+  const at::Tensor q = check_q(q_in);
+  const c10::Device dev = q.device();
+  const c10::DeviceGuard guard(dev);
+  no_grad({&q_in, &k_pool, &v_pool, s_aux ? &*s_aux : nullptr}, "paged_flash_decode_shared");
+  const at::Tensor k = kv_tensor(k_pool, "k_pool", dev, 4, "[num_pages, num_kv_heads, page_size, head_dim]");
+  const at::Tensor v = kv_tensor(v_pool, "v_pool", dev, 4, "[num_pages, num_kv_heads, page_size, head_dim]");
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2);
+  const int64_t P = k.size(0), Hkv = k.size(1), PS = k.size(2);
+  if (v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || k.size(3) != D)
+    raise(FSK_ERR_INVALID, "k_pool / v_pool shapes or types disagree with each other or with q");
+  if (page_size != PS)
+    raise(FSK_ERR_INVALID, "page_size=" + std::to_string(page_size) + " but the pools hold " + std::to_string(PS) +
+                               "-token pages");
+  on_device(block_table, "block_table", dev);
+  if (block_table.dim() != 2 || block_table.size(0) < B) raise(FSK_ERR_INVALID, "block_table must be [batch, max_blocks]");
+  at::Tensor bt = block_table.scalar_type() == at::kInt ? block_table : block_table.to(at::kInt);
+  if (bt.stride(1) != 1) bt = bt.contiguous();
+  const Lengths ln = lengths(seq_lens, "seq_lens", dev, false);  // (host lengths are copied to the device)
+  if (ln.t.numel() < B) raise(FSK_ERR_INVALID, "seq_lens must have one entry per sequence");
+  const auto sk = sinks(s_aux, Hq, dev);
+  const auto ks = scale(k_scale, "k_scale", dev), vs = scale(v_scale, "v_scale", dev);
+  const at::Tensor out = at::empty({B, Hq, D}, q.options().dtype(out_dtype(out_code, q)));
+  const int64_t max_blocks = bt.size(1);
+  if (B == 0) return out;  // (an empty tensor has no address to pass)
+  const int64_t nbytes = fsk_shared_workspace_bytes((int)B, (int)Hq, (int)Hkv, (int)D, max_blocks, (int)PS, shared_len);
+  const c10::DataPtr ws = workspace(nbytes, out);
+  check(fsk_decode_paged_shared(
+      q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.data_ptr(),
+      v.stride(0), v.stride(1), v.stride(2), bt.data_ptr<int32_t>(), bt.stride(0), (int)max_blocks,
+      ln.t.data_ptr<int32_t>(), shared_len, (int)P, (int)PS, static_cast<const float*>(ptr_or_null(sk)), (int)sink_mode,
+      static_cast<const float*>(ptr_or_null(ks)), static_cast<const float*>(ptr_or_null(vs)), out.data_ptr(),
+      out.stride(0), out.stride(1), (int)B, (int)Hq, (int)Hkv, (int)D, dtype_code(q.scalar_type(), "q"),
+      dtype_code(k.scalar_type(), "k_pool"), dtype_code(out.scalar_type(), "out_dtype"), softmax_scale(sm_scale, D),
+      ws.get(), nbytes, stream_ptr(stream)));
   return out;
 }
 
@@ -456,14 +509,6 @@ void kv_write(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& 
 // ---------------------------------------------------------------------------
 // Norm and rotation of query and key rows, to tensors or into the paged cache
 // ---------------------------------------------------------------------------
-// The kernels are not recorded: a call whose inputs want gradients is refused.
-void no_grad(std::initializer_list<const at::Tensor*> tensors, const char* what) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const at::Tensor* t : tensors)
-    if (t && t->defined() && t->requires_grad())
-      raise(kRuntime, std::string(what) + " has no backward pass: call it under torch.no_grad() or detach its inputs");
-}
-
 const at::Tensor* maybe(const c10::optional<at::Tensor>& t) { return t ? &*t : nullptr; }
 
 // A [n, H, D] tensor with rows the kernels can load, else a packed copy (an
@@ -792,6 +837,9 @@ PYBIND11_MODULE(_fsk_torch, m) {
         py::arg("seq_lens"), py::arg("page_size"), py::arg("s_aux"), py::arg("k_scale"), py::arg("v_scale"),
         py::arg("out_code"), py::arg("sink_mode"), py::arg("sm_scale"), py::arg("chunk_tokens"), py::arg("scores"),
         py::arg("stream"));
+  m.def("paged_shared", &paged_shared, py::arg("q"), py::arg("k_pool"), py::arg("v_pool"), py::arg("block_table"),
+        py::arg("seq_lens"), py::arg("page_size"), py::arg("shared_len"), py::arg("s_aux"), py::arg("k_scale"),
+        py::arg("v_scale"), py::arg("out_code"), py::arg("sink_mode"), py::arg("sm_scale"), py::arg("stream"));
   m.def("varlen", &varlen, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cu_seqlens"), py::arg("s_aux"),
         py::arg("k_scale"), py::arg("v_scale"), py::arg("out_code"), py::arg("sink_mode"), py::arg("sm_scale"),
         py::arg("chunk_tokens"), py::arg("scores"), py::arg("stream"));

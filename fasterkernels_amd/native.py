@@ -66,6 +66,9 @@ SIGNATURES = {
     "fsk_paged_gather": (_I, [_P, _L, _L, _L, _P, _L, _I, _P, _I, _I, _I, _I, _I, _I, _P, _P]),
     "fsk_paged_write": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _P, _L, _L, _L, _P, _L, _L, _L, _I, _I,
                              _I, _I, _I, _I, _P, _P, _P, _L, _P, _L, _P]),
+    "fsk_shared_workspace_bytes": (_L, [_I, _I, _I, _I, _L, _I, _L]),
+    "fsk_decode_paged_shared": (_I, [_P, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _I, _P, _L, _I, _I, _P, _I, _P,
+                                     _P, _P, _L, _L, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P]),
     "fsk_qk_norm_rope": (_I, [_P, _L, _L, _P, _L, _L, _L, _P, _L, _P, _L, _L, _I, _I, _I, _P, _P, _P, _I, _F, _P,
                               _L, _L, _P, _L, _L, _I, _I, _I, _I, _P]),
     "fsk_paged_write_rope": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _P, _L, _P, _L, _L, _I, _I, _I, _P, _P,

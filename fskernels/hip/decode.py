@@ -321,6 +321,29 @@ def paged_flash_decode(q, k_pool, v_pool, block_table, seq_lens, page_size, *, s
     return out if scores is None else (out, scores)
 
 
+def paged_flash_decode_shared(q, k_pool, v_pool, block_table, seq_lens, page_size, shared_len, *, s_aux=None,
+                              k_scale=None, v_scale=None, out_dtype: torch.dtype | None = None,
+                              sink_mode: str = "linear", sm_scale: float | None = None):
+    """``paged_flash_decode`` of a batch whose sequences begin with the same
+    ``shared_len`` tokens in the same pages (a system prompt, a document, many
+    samples of one prompt), attended once for all of them.
+
+    The caller vouches that the first ``shared_len // page_size`` entries of
+    every block-table row are the first row's (``PagedKVCache.shared_prefix_len``
+    gives such a length); these pages' K and V are then read once for the batch
+    and multiplied with all its queries at once, each sequence's other tokens
+    are attended as paged_flash_decode does, and the two parts are merged.  The
+    result is paged_flash_decode's, which has no counterpart of this in the
+    reference; a sequence shorter than ``shared_len`` attends its first
+    ``seq_lens[b]`` tokens.  ``shared_len`` is a host number (part of a captured
+    graph); host lengths are copied to the device.  Inference only: inputs that
+    want gradients are refused.
+    """
+    return nat.ext().paged_shared(q, k_pool, v_pool, block_table, seq_lens, int(page_size), int(shared_len), s_aux,
+                                  _scale_tensor(k_scale, q), _scale_tensor(v_scale, q), _out_code(out_dtype),
+                                  _sink_mode(sink_mode), _sm(sm_scale), _stream(q))
+
+
 # ---------------------------------------------------------------------------
 # debug exports
 # ---------------------------------------------------------------------------

@@ -206,6 +206,36 @@ FSK_API int fsk_decode_paged_noalloc(const void *q, int64_t q_stride_b, int64_t 
                      int q_dtype, int kv_dtype, int out_dtype, float sm_scale,
                      int chunk_tokens, void *stream);
 
+/* Paged decode of a batch whose sequences begin with the same tokens in the
+ * same pages.  No counterpart in the reference (its paged kernel reads a shared
+ * prompt's pages once for every sequence).
+ * The result of fsk_decode_paged with the same arguments, provided that the
+ * first shared_len / page_size entries (rounded down) of every sequence's
+ * block-table row are those of the first sequence's row, which are the ones
+ * read: the attention over these pages is computed for all sequences at once
+ * (K and V read once for the batch, matrix products instead of one
+ * matrix-vector product per sequence), each sequence's other tokens as
+ * fsk_decode_paged does, and the two merged.  Sequences shorter than shared_len
+ * attend their first seq_lens[b] tokens, as there; whatever lies past a
+ * sequence's end does not reach its output.  shared_len in [0, max_blocks *
+ * page_size], a host value (under graph capture part of the graph).  The
+ * workspace holds fsk_shared_workspace_bytes(...) bytes. */
+FSK_API int64_t fsk_shared_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                     int64_t max_blocks, int page_size, int64_t shared_len);
+FSK_API int fsk_decode_paged_shared(const void *q, int64_t q_stride_b, int64_t q_stride_h,
+                     const void *k_pool, int64_t k_stride_p, int64_t k_stride_h,
+                     int64_t k_stride_t,
+                     const void *v_pool, int64_t v_stride_p, int64_t v_stride_h,
+                     int64_t v_stride_t,
+                     const int32_t *block_table, int64_t bt_stride_b, int max_blocks,
+                     const int32_t *seq_lens, int64_t shared_len, int num_pages, int page_size,
+                     const float *s_aux, int sink_mode,
+                     const float *k_scale, const float *v_scale,
+                     void *out, int64_t o_stride_b, int64_t o_stride_h,
+                     int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                     int q_dtype, int kv_dtype, int out_dtype, float sm_scale,
+                     void *workspace, int64_t workspace_bytes, void *stream);
+
 /* Block scores: the varlen / paged decode plus, per sequence b, query head h
  * and 128-token block j of the sequence, the largest final attention
  * probability of a token of that block:
