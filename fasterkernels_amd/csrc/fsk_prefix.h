@@ -39,6 +39,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4_w;
+typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 
 template <bool kBf16>
 __device__ __forceinline__ f32x16 mfma32x32x16(u32x4 a, u32x4 b, f32x16 c) {
@@ -63,24 +64,25 @@ __device__ __forceinline__ u32x2 lds_read_tr16(uint32_t off) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)off));
 }
 
-// Tile geometry.  K and V tiles of kTile tokens lie in LDS as 16-bit rows (e4m3
+// Tile geometry.  K and V tiles of 64 tokens lie in LDS as 16-bit rows (e4m3
 // codes are widened on the way in: both widenings are exact), each row's
 // 16-byte chunks in an order that spreads the operand reads over the banks.
+// LDS: two K tiles, then two V tiles.
 template <int D>
 struct PrefixTile {
-  static constexpr int kTile = D <= 128 ? 64 : 32;
+  static constexpr int kTile = 64;
   static constexpr int kRow = 2 * D;             // bytes
   static constexpr int kChunks = kRow / 16;
   static constexpr int kPlane = kTile * kRow;    // one tile of K or V
+  static constexpr int kBlock = 32 * kRow;       // a score block's rows
   static constexpr int kHalves = kTile / 16;     // 16-token pieces, each inside one page
-  static constexpr int kBlocks = kTile / 32;     // 32-token score blocks
+  static constexpr int kPerEu = D <= 128 ? 2 : 1;  // waves a SIMD the registers are sized for
 };
-// V chunk m of row R is stored at m ^ v_swizzle(R): the transposing reads take
-// 8 consecutive rows x 64 bytes, which land on all banks twice (512 bytes over
-// 64 banks of 4).
+// V chunk m of row R is stored at m ^ v_swizzle(R): a transposing read takes 4
+// rows x 64 bytes a half-wave, which land on different banks (64 of 4 bytes).
 template <int kChunks>
 __device__ __forceinline__ int v_swizzle(int row) {
-  return kChunks >= 16 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
+  return kChunks >= 16 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
 }
 
 // One work item: kWaves x 32 query rows of one KV head against `chunk` tiles.
@@ -91,21 +93,26 @@ __device__ __forceinline__ int v_swizzle(int row) {
 // given token 16 s + 4 h + e (e < 4) or 16 s + 4 h + 4 + e, which is where the
 // score block left P, so P needs no movement; V^T comes from LDS through the
 // transposing read (16 lanes read 4 token rows of 16 dims, lane i gets dim i).
+//
+// Three score blocks are in work at once, so that matrix and vector instructions
+// of one wave overlap (a wave's MFMA holds the matrix pipe for 32 cycles, in
+// which it issues up to five vector instructions): while block i goes through
+// the softmax, the products of block i + 1 and the values of block i - 1 are
+// multiplied.  Tile t's K is therefore needed one stage before its V, and their
+// buffers are refilled at different times: with one barrier a tile, K of tile
+// t + 2 and V of tile t + 1 are loaded while blocks 2 t + 1 and 2 t + 2 go through.
 template <int D, bool kQBf16, bool kVBf16, bool kFp8, int kWaves>
-__global__ __launch_bounds__(64 * kWaves) void prefix_kernel(PrefixParams p) {
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(PrefixTile<D>::kPerEu, PrefixTile<D>::kPerEu)))
+void prefix_kernel(PrefixParams p) {
   using T = PrefixTile<D>;
   constexpr int kSteps = D / 16;    // QK k-steps
   constexpr int kDb = D / 32;       // output blocks of 32 dims
-  constexpr int kPv = T::kTile / 16;  // PV k-steps
-  extern __shared__ __attribute__((aligned(16))) uint8_t s_prefix[];  // [2 buffers][K, V]
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_prefix[];  // K, K, V, V
   const uint32_t lds = (uint32_t)(uintptr_t)s_prefix;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = uniform((int)threadIdx.x / kWave);
   const int h = lane >> 5, c = lane & 31;
 
-  if (blockIdx.x == 0) {
-    for (int b = threadIdx.x; b < p.B; b += 64 * kWaves) p.own_lens[b] = max(clampi(p.lens[b], 0, p.max_len) - p.tokens, 0);
-  }
   // Row tiles of one (chunk, head) on one XCD, one after the other: they read
   // the same K and V through its L2.
   const uint32_t xcd = blockIdx.x & 7, in_xcd = blockIdx.x >> 3;
@@ -117,52 +124,48 @@ __global__ __launch_bounds__(64 * kWaves) void prefix_kernel(PrefixParams p) {
   const int kvh = (int)unit - jc * p.Hkv;
   const int tile0 = jc * p.chunk, tile1 = min(tile0 + p.chunk, p.tiles);
 
-  // ---- this lane's query column
+  // ---- first loads, in flight together: the pages of the wave's first 64
+  // 16-token pieces (lane i: piece base + i), the query rows and the lengths.
+  // The wave stages pieces wave, wave + kWaves, .. of a tile.
+  constexpr int kPieces = T::kHalves / kWaves;
+  int win_base = tile0 * T::kHalves;
+  auto page_of = [&](int piece) {
+    const int t = min(16 * piece, p.tokens - 1);  // (pieces past the prefix are not staged)
+    return p.pages[fdiv((uint32_t)t, p.page)];
+  };
+  const int first_page = page_of(win_base + lane);
   const int row0 = (rt * kWaves + wave) * 32;
   const bool live = row0 < p.rows;                // any column of the wave is a query row
   const int row = min(row0 + c, p.rows - 1);
   const bool row_ok = row0 + c < p.rows;
   const int b = (int)fdiv((uint32_t)row, p.g_div);
-  const int lim = row_ok ? min(clampi(p.lens[b], 0, p.max_len), p.tokens) : p.tokens;  // shared tokens it attends
   u32x4 qop[kSteps];
   {
     const uint8_t* qrow = p.q + (int64_t)b * p.q_sb + (int64_t)(kvh * p.G + (row - b * p.G)) * p.q_sh;
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const u32x4 x = *(const u32x4*)(qrow + 32 * i + 16 * h);
-      qop[i] = row_ok ? x : u32x4{0, 0, 0, 0};
-    }
+    for (int i = 0; i < kSteps; ++i) qop[i] = *(const u32x4*)(qrow + 32 * i + 16 * h);
   }
-  const float sscale = p.score_scale * (kFp8 ? *p.k_scale : 1.0f);
-  int lim_min = lim;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o));
-  lim_min = uniform(lim_min);
+  float sscale = p.score_scale * (kFp8 ? *p.k_scale : 1.0f);
 
-  // ---- staging: 16-token pieces dealt to the waves.  Pages of the next 64
-  // pieces in one register (lane i: piece base + i).
+  // ---- staging
   const uint8_t* kbase = p.k + (int64_t)kvh * p.k_sh;
   const uint8_t* vbase = p.v + (int64_t)kvh * p.v_sh;
-  int win = 0, win_base = -64;
-  auto piece_at = [&](int piece, int64_t& ko, int64_t& vo, bool& ok) {  // byte offsets of a piece's first rows
-    if (piece - win_base >= 64) {  // (pieces come in order)
-      win_base = piece;
-      const int t = 16 * (piece + lane);
-      win = t < p.tokens ? clampi(p.pages[fdiv((uint32_t)t, p.page)], 0, p.num_pages - 1) : 0;
-    }
-    const int t = 16 * piece;
-    ok = t < p.tokens;
-    const int page = __builtin_amdgcn_readlane(win, piece - win_base);
-    const int off = t - (int)fdiv((uint32_t)t, p.page) * (int)p.page.d;
-    ko = (int64_t)page * p.k_sp + (int64_t)off * p.k_st;
-    vo = (int64_t)page * p.v_sp + (int64_t)off * p.v_st;
+  // Byte offsets of the pieces' first rows, in the lanes.
+  int64_t k_piece, v_piece;
+  auto place = [&](int page) {
+    page = clampi(page, 0, p.num_pages - 1);
+    const int t = 16 * (win_base + lane);
+    const int row_in = t - (int)fdiv((uint32_t)t, p.page) * (int)p.page.d;
+    k_piece = (int64_t)page * p.k_sp + (int64_t)row_in * p.k_st;
+    v_piece = (int64_t)page * p.v_sp + (int64_t)row_in * p.v_st;
   };
-  constexpr int kPieces = (T::kHalves + kWaves - 1) / kWaves;  // of this wave, per tile
+  place(first_page);
   // 16-bit: DMA, 1 KB (64 / kChunks rows) a load.  e4m3: 16 codes a lane and load,
   // 1 KB = 1024 / D rows, kept in registers until the buffer is free.
   constexpr int kDma = 16 * T::kRow / 1024;
-  constexpr int kCodeLoads = 16 * D / 1024 > 0 ? 16 * D / 1024 : 1;
-  u32x4 codes[kFp8 ? 2 * kPieces * kCodeLoads : 1];
+  constexpr int kCodeLoads = 16 * D / 1024;
+  constexpr int kCodes = kFp8 ? kPieces * kCodeLoads : 1;
+  u32x4 k_codes[kCodes], v_codes[kCodes];
   int k_off[kDma], v_off[kDma];
   if constexpr (!kFp8) {
 #pragma unroll
@@ -173,110 +176,188 @@ __global__ __launch_bounds__(64 * kWaves) void prefix_kernel(PrefixParams p) {
       v_off[r] = R * (int)p.v_st + 16 * (m ^ v_swizzle<T::kChunks>(R));
     }
   }
-  auto load = [&](int tile, uint32_t buf) {
+  // This wave's pieces of a tile's K or V into a plane (16-bit), or into registers
+  // (e4m3) from which put() widens them into it.  Pieces past the prefix read as zeros.
+  auto load = [&](const uint8_t* base, int64_t at, int64_t st, const int (&off)[kDma], u32x4 (&codes)[kCodes], int tile,
+                  uint32_t plane) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int hp = wave + i * kWaves;  // piece of the tile
-      if (T::kHalves % kWaves != 0 && hp >= T::kHalves) break;
-      int64_t ko, vo;
-      bool ok;
-      piece_at(tile * T::kHalves + hp, ko, vo, ok);
-      // (pieces past the prefix read as zeros)
-      const auto rk = make_rsrc(kbase + ko, ok ? 15 * (int)p.k_st + (kFp8 ? D : 2 * D) : 0);
-      const auto rv = make_rsrc(vbase + vo, ok ? 15 * (int)p.v_st + (kFp8 ? D : 2 * D) : 0);
-      if constexpr (!kFp8) {
+      const int piece = tile * T::kHalves + hp;
+      const int from = (piece - win_base) & 63;
+      const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, from);
+      const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)at >> 32), from);
+      const auto rs = make_rsrc(base + (int64_t)(((uint64_t)hi << 32) | lo),
+                                16 * piece < p.tokens ? 15 * (int)st + (kFp8 ? D : 2 * D) : 0);
 #pragma unroll
-        for (int r = 0; r < kDma; ++r) {
-          lds_dma16(rk, buf + hp * 16 * T::kRow + r * 1024, k_off[r]);
-          lds_dma16(rv, buf + T::kPlane + hp * 16 * T::kRow + r * 1024, v_off[r]);
-        }
-      } else {
-#pragma unroll
-        for (int r = 0; r < kCodeLoads; ++r) {
+      for (int r = 0; r < (kFp8 ? kCodeLoads : kDma); ++r) {
+        if constexpr (!kFp8) {
+          lds_dma16(rs, plane + hp * 16 * T::kRow + r * 1024, off[r]);
+        } else {
           const int R = r * (1024 / D) + lane * 16 / D, d0 = lane * 16 % D;
-          const auto x = buf_load<16>(rk, R * (int)p.k_st + d0), y = buf_load<16>(rv, R * (int)p.v_st + d0);
-          codes[2 * (i * kCodeLoads + r)] = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
-          codes[2 * (i * kCodeLoads + r) + 1] = u32x4{y.w[0], y.w[1], y.w[2], y.w[3]};
+          const auto x = buf_load<16>(rs, R * (int)st + d0);
+          codes[i * kCodeLoads + r] = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
         }
       }
     }
   };
-  // e4m3: the loaded codes, widened, into the buffer.
-  auto store = [&](uint32_t buf) {
+  auto put = [&](auto is_v, const u32x4 (&codes)[kCodes], uint32_t plane) {
     if constexpr (kFp8) {
+      constexpr bool kV = decltype(is_v)::value;
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int hp = wave + i * kWaves;
-        if (T::kHalves % kWaves != 0 && hp >= T::kHalves) break;
+      for (int i = 0; i < kPieces; ++i)
 #pragma unroll
         for (int r = 0; r < kCodeLoads; ++r) {
           const int R = r * (1024 / D) + lane * 16 / D, m = lane * 16 % D / 8;
-          const u32x4 kc = codes[2 * (i * kCodeLoads + r)], vc = codes[2 * (i * kCodeLoads + r) + 1];
+          const int swz = kV ? v_swizzle<T::kChunks>(R) : k_swizzle<T::kChunks>(R);
+          const u32x4 x = codes[i * kCodeLoads + r];
+          const uint32_t at = plane + ((wave + i * kWaves) * 16 + R) * T::kRow;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const u32x2 k0 = e4m3x4_to<kQBf16>(kc[2 * e]), k1 = e4m3x4_to<kQBf16>(kc[2 * e + 1]);
-            const u32x2 v0 = e4m3x4_to<kVBf16>(vc[2 * e]), v1 = e4m3x4_to<kVBf16>(vc[2 * e + 1]);
-            const uint32_t at = buf + (hp * 16 + R) * T::kRow;
-            *(lds_u32x4_w*)(uintptr_t)(at + 16 * ((m + e) ^ k_swizzle<T::kChunks>(R))) = u32x4{k0[0], k0[1], k1[0], k1[1]};
-            *(lds_u32x4_w*)(uintptr_t)(at + T::kPlane + 16 * ((m + e) ^ v_swizzle<T::kChunks>(R))) =
-                u32x4{v0[0], v0[1], v1[0], v1[1]};
+            const u32x2 lo = e4m3x4_to<kV ? kVBf16 : kQBf16>(x[2 * e]), hi = e4m3x4_to<kV ? kVBf16 : kQBf16>(x[2 * e + 1]);
+            *(lds_u32x4_w*)(uintptr_t)(at + 16 * ((m + e) ^ swz)) = u32x4{lo[0], lo[1], hi[0], hi[1]};
           }
         }
-      }
     }
   };
+  // (the window moves on when K, which runs a tile ahead of V, leaves it; V's pieces
+  // of the tile before are still in it: 64 pieces are 16 tiles, kept from the
+  // tile before the one that moves it)
+  auto window = [&](int tile) {
+    if ((tile + 1) * T::kHalves - win_base > 64) {
+      win_base = (tile - 1) * T::kHalves;
+      place(page_of(win_base + lane));
+    }
+  };
+  auto load_k = [&](int tile) {
+    window(tile);
+    load(kbase, k_piece, p.k_st, k_off, k_codes, tile, lds + ((tile - tile0) & 1) * T::kPlane);
+  };
+  auto load_v = [&](int tile) {
+    load(vbase, v_piece, p.v_st, v_off, v_codes, tile, lds + (2 + ((tile - tile0) & 1)) * T::kPlane);
+  };
+  auto put_k = [&](int tile) { put(std::false_type{}, k_codes, lds + ((tile - tile0) & 1) * T::kPlane); };
+  auto put_v = [&](int tile) { put(std::true_type{}, v_codes, lds + (2 + ((tile - tile0) & 1)) * T::kPlane); };
+  load_k(tile0);
+  load_v(tile0);
 
-  // ---- operand addresses: XOR with a constant picks the chunk
-  const uint32_t k_lane = c * T::kRow + 16 * (h ^ k_swizzle<T::kChunks>(c));
-  const int vj = lane & 15, vr = 4 * h + vj / 4;
-  const uint32_t v_lane = T::kPlane + vr * T::kRow +
-                          16 * ((2 * (c >> 4) + (vj & 3) / 2) ^ v_swizzle<T::kChunks>(vr)) + 8 * (vj & 1);
+  const int len = p.lens[b];
+  // Whether a row of the workgroup's tile ends inside this chunk (every wave looks
+  // at all of them: the waves take one path, which holds barriers).
+  const int first = tile0 * T::kTile, end = min(tile1 * T::kTile, p.tokens);  // the chunk's tokens
+  bool ends_inside = false;
+  for (int r = lane; r < 32 * kWaves; r += kWave) {
+    const int rr = min(rt * 32 * kWaves + r, p.rows - 1);
+    const int l = p.lens[fdiv((uint32_t)rr, p.g_div)];
+    ends_inside = ends_inside || (l > first && l < end);
+  }
+  const int lim = row_ok ? min(clampi(len, 0, p.max_len), p.tokens) : p.tokens;  // shared tokens the column attends
+  const bool ragged = __builtin_amdgcn_ballot_w64(ends_inside) != 0;
+  // The scale's sign goes to Q (exactly), so that the largest product is the
+  // largest score; a scale of zero becomes the smallest normal number, which
+  // scores every finite product as zero and keeps masked ones at -inf.
+  {
+    const uint32_t sign = sscale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qop[i][e] = row_ok ? qop[i][e] ^ sign : 0u;
+  }
+  sscale = fabsf(sscale) < 1.17549435e-38f ? 1.17549435e-38f : fabsf(sscale);
 
-  float m_ref = -INFINITY, l_run = 0.f;
+  // ---- operand addresses: the chunk of a k-step (dim block) is an XOR away, tile
+  // row and buffer a constant offset
+  uint32_t k_at[kSteps], v_at[kDb];
+  {
+    const int vj = lane & 15, vr = 4 * h + vj / 4;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+      k_at[i] = lds + ((c * T::kRow + 16 * (h ^ k_swizzle<T::kChunks>(c))) ^ (32 * i));
+#pragma unroll
+    for (int d = 0; d < kDb; ++d)
+      v_at[d] = lds + 2 * T::kPlane + ((vr * T::kRow + 16 * ((2 * (c >> 4) + (vj & 3) / 2) ^ v_swizzle<T::kChunks>(vr)) +
+                                    8 * (vj & 1)) ^ (64 * d));
+  }
+  auto k_operand = [&](uint32_t off, int i) { return *(lds_u32x4*)((lds_u8*)(uintptr_t)k_at[i] + off); };
+  auto v_operand = [&](uint32_t off, int st, int d) {
+    const u32x2 lo = lds_read_tr16(v_at[d] + (off + st * 16 * T::kRow));
+    const u32x2 hi = lds_read_tr16(v_at[d] + (off + st * 16 * T::kRow + 8 * T::kRow));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+
+  auto turn_k = [&](int by) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) k_at[i] += by;
+  };
+  auto turn_v = [&](int by) {
+#pragma unroll
+    for (int d = 0; d < kDb; ++d) v_at[d] += by;
+  };
+
+  float m_ref = -INFINITY, m_max = -INFINITY, l_run = 0.f;
   f32x16 acc[kDb];
 #pragma unroll
   for (int d = 0; d < kDb; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
 
-  auto compute = [&](int tile, uint32_t buf) {
-    const int t0 = tile * T::kTile;
-    // scores, log2 domain
-    f32x16 s[T::kBlocks];
+  // off: the block's offset in the two K (V) planes
+  auto scores = [&](uint32_t off) {
+    f32x16 s;
 #pragma unroll
-    for (int tb = 0; tb < T::kBlocks; ++tb) {
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[tb][i] = 0.f;
+    for (int i = 0; i < kSteps; ++i) s = mfma32x32x16<kQBf16>(k_operand(off, i), qop[i], s);
+    return s;
+  };
+  // Block's reference point (log2 domain).  The exponentials are taken relative
+  // to m_ref, which follows the running maximum only when that has grown by
+  // more than 2^8: the sums stay in fp32 and P below 2^8 keeps its relative
+  // precision in 16 bits, while rescaling is left out of nearly every block.
+  auto reference = [&](const f32x16& s) {
+    float mt = s[0];
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const u32x4 kop = *(lds_u32x4*)(uintptr_t)(buf + tb * 32 * T::kRow + (k_lane ^ (32 * i)));
-        s[tb] = mfma32x32x16<kQBf16>(kop, qop[i], s[tb]);
-      }
+    for (int i = 1; i < 16; ++i) mt = fmaxf(mt, s[i]);
+    mt = half_max(mt) * sscale;
+    m_max = fmaxf(m_max, mt);
+    return mt > m_ref + 8.f ? mt : m_ref;
+  };
+  // P^T operands of a block's two k-steps relative to m_new, and the sum of P;
+  // bf16 P as hi + lo parts, as in the split kernel.
+  struct Weights {
+    u32x4 hi[2], lo[2];
+    float sum;
+  };
+  // Two weights, rounded into operands, and added to their sum.
+  auto weight_pair = [&](uint32_t& hi, uint32_t& lo, float& sum, float a, float z) {
+    if constexpr (kVBf16) {
+      hi = pack_bf16x2(a, z);
+      lo = pack_bf16x2(a - bf16_lo_to_f32(hi), z - bf16_hi_to_f32(hi));
+      sum += a;
+      sum += z;
+    } else {
+      // the sum of the weights as they are multiplied (fp32 sum of the f16 pair)
+      hi = pack_f16x2(a, z);
+      sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, hi), f16x2{(f16)1.f, (f16)1.f}, sum, false);
     }
+  };
+  auto weights = [&](const f32x16& s, float m_new) {
+    Weights w;
+    w.sum = 0.f;
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
 #pragma unroll
-    for (int tb = 0; tb < T::kBlocks; ++tb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[tb][i] *= sscale;
-    if (t0 + T::kTile > lim_min) {
-#pragma unroll
-      for (int tb = 0; tb < T::kBlocks; ++tb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (t0 + 32 * tb + 8 * (i / 4) + 4 * h + i % 4 >= lim) s[tb][i] = -INFINITY;
+    for (int j = 0; j < 8; ++j) {
+      uint32_t hi, lo = 0;
+      weight_pair(hi, lo, w.sum, __builtin_amdgcn_exp2f(fmaf(s[2 * j], sscale, -m_use)),
+                  __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], sscale, -m_use)));
+      w.hi[j / 4][j % 4] = hi;
+      w.lo[j / 4][j % 4] = lo;
     }
-    float mt = s[0][0];
-#pragma unroll
-    for (int tb = 0; tb < T::kBlocks; ++tb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[tb][i]);
-    mt = half_max(mt);
-    // The exponentials are taken relative to m_ref, which follows the running
-    // maximum only when that has grown by more than 2^8: the sums stay in fp32
-    // and P below 2^8 keeps its relative precision in 16 bits, while the
-    // rescaling of the accumulators is left out of nearly every tile.
-    if (__builtin_amdgcn_ballot_w64(mt > m_ref + 8.f) != 0) {
-      const float m_new = fmaxf(m_ref, mt);
-      const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_ref - m_new);
+    return w;
+  };
+  auto rescale = [&](float m_new) {
+    if (__builtin_amdgcn_ballot_w64(m_new != m_ref) != 0) {
+      const float alpha = m_new != m_ref ? __builtin_amdgcn_exp2f(m_ref - m_new) : 1.f;
       l_run *= alpha;
 #pragma unroll
       for (int d = 0; d < kDb; ++d)
@@ -284,51 +365,120 @@ __global__ __launch_bounds__(64 * kWaves) void prefix_kernel(PrefixParams p) {
         for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
       m_ref = m_new;
     }
-    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-    // P^T operands; bf16 P as hi + lo parts, as in the split kernel
-    u32x4 pop[kPv], plo[kVBf16 ? kPv : 1];
+  };
+  auto values = [&](uint32_t off, const Weights& w) {
 #pragma unroll
-    for (int st = 0; st < kPv; ++st) {
-      float pv[8];
+    for (int st = 0; st < 2; ++st)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        pv[e] = __builtin_amdgcn_exp2f(s[st / 2][8 * (st & 1) + e] - m_use);
-        l_run += pv[e];
+      for (int d = 0; d < kDb; ++d) {
+        const u32x4 vop = v_operand(off, st, d);
+        acc[d] = mfma32x32x16<kVBf16>(vop, w.hi[st], acc[d]);
+        if constexpr (kVBf16) acc[d] = mfma32x32x16<true>(vop, w.lo[st], acc[d]);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (kVBf16) {
-          const uint32_t hi = pack_bf16x2(pv[2 * e], pv[2 * e + 1]);
-          pop[st][e] = hi;
-          plo[st][e] = pack_bf16x2(pv[2 * e] - bf16_lo_to_f32(hi), pv[2 * e + 1] - bf16_hi_to_f32(hi));
-        } else {
-          pop[st][e] = pack_f16x2(pv[2 * e], pv[2 * e + 1]);
-        }
+  };
+  // One stage: products of the next block into s_next, softmax of s, values of
+  // the block before (weights w_prev).  Returns s's weights; m: their reference.
+  // Written slot by slot, one matrix instruction with the operand reads of two
+  // slots on and its share of the softmax in each (left to itself the compiler
+  // puts the reads next to their use and the exponentials in a row): the steps
+  // are the maximum of 8 and 8 scores, the reference, then pair by pair the
+  // exponent, the exponential and the rounding, one step apart.
+  auto stage = [&](auto qk, auto pv, uint32_t k_blk, uint32_t v_blk, f32x16& s_next, const f32x16& s,
+                   const Weights& w_prev, float& m) {
+    constexpr bool kQk = decltype(qk)::value, kPv = decltype(pv)::value;
+    static_assert(kSteps == 2 * kDb, "a k-step of QK for every V operand");
+    constexpr int kPer = (kQk ? 1 : 0) + (kPv ? (kVBf16 ? 2 : 1) : 0);
+    constexpr int kSlots = kSteps * kPer, kTimes = 13, kAhead = 2;
+    u32x4 kop[kSteps], vop[kSteps];
+    float x[16], mt = -INFINITY, m_use = 0.f;
+    Weights w;
+    w.sum = 0.f;
+    auto step = [&](int t) {
+      if (t == 0 || t == 1) {
+        float a = fmaxf(fmaxf(s[8 * t], s[8 * t + 1]), s[8 * t + 2]);
+        a = fmaxf(fmaxf(a, s[8 * t + 3]), s[8 * t + 4]);
+        a = fmaxf(fmaxf(a, s[8 * t + 5]), s[8 * t + 6]);
+        mt = fmaxf(fmaxf(a, s[8 * t + 7]), mt);
+        asm volatile("" : "+v"(mt));  // (here and below: keeps the step in its slot)
       }
-    }
-    auto v_operand = [&](int st, int d) {
-      const uint32_t at = buf + st * 16 * T::kRow + (v_lane ^ (64 * d));
-      const u32x2 lo = lds_read_tr16(at), hi = lds_read_tr16(at + 8 * T::kRow);
-      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+      if (t == 2) {
+        mt = half_max(mt) * sscale;
+        m_max = fmaxf(m_max, mt);
+        m = mt > m_ref + 8.f ? mt : m_ref;
+        m_use = m == -INFINITY ? 0.f : m;
+        asm volatile("" : "+v"(m_use));
+      }
+      if (t >= 3 && t < 11) {
+        const int j = 2 * (t - 3);
+        x[j] = fmaf(s[j], sscale, -m_use);
+        x[j + 1] = fmaf(s[j + 1], sscale, -m_use);
+        asm volatile("" : "+v"(x[j]), "+v"(x[j + 1]));
+      }
+      if (t >= 4 && t < 12) {
+        const int j = 2 * (t - 4);
+        x[j] = __builtin_amdgcn_exp2f(x[j]);
+        x[j + 1] = __builtin_amdgcn_exp2f(x[j + 1]);
+        asm volatile("" : "+v"(x[j]), "+v"(x[j + 1]));
+      }
+      if (t >= 5) {
+        const int j = t - 5;
+        uint32_t hi, lo = 0;
+        weight_pair(hi, lo, w.sum, x[2 * j], x[2 * j + 1]);
+        asm volatile("" : "+v"(hi), "+v"(lo), "+v"(w.sum));
+        w.hi[j / 4][j % 4] = hi;
+        w.lo[j / 4][j % 4] = lo;
+      }
     };
-    if (lim_min >= min(t0 + T::kTile, p.tokens)) {
+    auto read = [&](int i) {
+      if (i >= kSteps) return;
+      if constexpr (kQk) kop[i] = k_operand(k_blk, i);
+      if constexpr (kPv) vop[i] = v_operand(v_blk, i / kDb, i % kDb);
+    };
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int st = 0; st < kPv; ++st)
+    for (int i = 0; i < kAhead; ++i) read(i);
+    if constexpr (kQk) {
 #pragma unroll
-        for (int d = 0; d < kDb; ++d) {
-          const u32x4 vop = v_operand(st, d);
-          acc[d] = mfma32x32x16<kVBf16>(vop, pop[st], acc[d]);
-          if constexpr (kVBf16) acc[d] = mfma32x32x16<true>(vop, plo[st], acc[d]);
-        }
-    } else {
-      // Columns that end inside the prefix: V rows past a column's end may hold
-      // anything, and 0 x inf is NaN, so the tile is multiplied once per
-      // different end, with V's rows zeroed past it, and only the columns of
-      // that end take the sum.
+      for (int i = 0; i < 16; ++i) s_next[i] = 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < kSlots; ++n) {
+      const int i = n / kPer, which = n % kPer;
+      __builtin_amdgcn_sched_barrier(0);
+      if (kQk && which == 0) s_next = mfma32x32x16<kQBf16>(kop[i], qop[i], s_next);
+      if constexpr (kPv) {
+        if (which == kPer - (kVBf16 ? 2 : 1)) acc[i % kDb] = mfma32x32x16<kVBf16>(vop[i], w_prev.hi[i / kDb], acc[i % kDb]);
+        if (kVBf16 && which == kPer - 1) acc[i % kDb] = mfma32x32x16<true>(vop[i], w_prev.lo[i / kDb], acc[i % kDb]);
+      }
+      if (which == 0) read(i + kAhead);
+#pragma unroll
+      for (int t = n * kTimes / kSlots; t < (n + 1) * kTimes / kSlots; ++t) step(t);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    return w;
+  };
+  // A tile whose tokens do not all count for every column (columns that end
+  // inside the prefix, the prefix's last tile).  V rows past a column's end may
+  // hold anything, and 0 x inf is NaN, so each block is multiplied once per
+  // different end, with V's rows zeroed past it, and only the columns of that
+  // end take the sum.
+  auto compute_ends = [&](int tile) {
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb) {
+      const uint32_t off = ((tile - tile0) & 1) * T::kPlane + tb * T::kBlock;
+      const int t0 = tile * T::kTile + 32 * tb;
+      f32x16 s = scores(off);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (t0 + 8 * (i / 4) + 4 * h + i % 4 >= lim) s[i] = -INFINITY;
+      const float m_new = reference(s);
+      const Weights w = weights(s, m_new);
+      rescale(m_new);
+      l_run += w.sum;
       uint64_t todo = __builtin_amdgcn_ballot_w64(lim > t0);
       while (todo) {
-        const int end = __builtin_amdgcn_readlane(lim, __builtin_ctzll(todo));
-        const bool mine = lim == end;
+        const int last = __builtin_amdgcn_readlane(lim, __builtin_ctzll(todo));
+        const bool mine = lim == last;
         todo &= ~__builtin_amdgcn_ballot_w64(mine);
 #pragma unroll
         for (int d = 0; d < kDb; ++d) {
@@ -336,16 +486,15 @@ __global__ __launch_bounds__(64 * kWaves) void prefix_kernel(PrefixParams p) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) sum[i] = 0.f;
 #pragma unroll
-          for (int st = 0; st < kPv; ++st) {
-            u32x4 vop = v_operand(st, d);
+          for (int st = 0; st < 2; ++st) {
+            u32x4 vop = v_operand(off, st, d);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {  // dword e: tokens t, t + 1
               const int t = t0 + 16 * st + 4 * h + 8 * (e >> 1) + 2 * (e & 1);
-              const uint32_t keep = (t < end ? 0xffffu : 0u) | (t + 1 < end ? 0xffff0000u : 0u);
-              vop[e] &= keep;
+              vop[e] &= (t < last ? 0xffffu : 0u) | (t + 1 < last ? 0xffff0000u : 0u);
             }
-            sum = mfma32x32x16<kVBf16>(vop, pop[st], sum);
-            if constexpr (kVBf16) sum = mfma32x32x16<true>(vop, plo[st], sum);
+            sum = mfma32x32x16<kVBf16>(vop, w.hi[st], sum);
+            if constexpr (kVBf16) sum = mfma32x32x16<true>(vop, w.lo[st], sum);
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[d][i] += mine ? sum[i] : 0.f;
@@ -354,35 +503,116 @@ __global__ __launch_bounds__(64 * kWaves) void prefix_kernel(PrefixParams p) {
     }
   };
 
-  // ---- tiles: while one is computed, the next one's loads are in flight.  One
-  // barrier a tile: past it every wave's part of the tile is in LDS, and every
-  // wave has done with the other buffer.
-  load(tile0, lds);
-  store(lds);
-  for (int tile = tile0; tile < tile1; ++tile) {
-    const uint32_t cur = lds + (uint32_t)((tile - tile0) & 1) * (2 * T::kPlane);
-    const uint32_t nxt = lds + (uint32_t)((tile - tile0 + 1) & 1) * (2 * T::kPlane);
+  // ---- tiles.  Past a barrier every wave's part of what was loaded before it is in
+  // LDS, and every wave has done with what it read before it.
+  auto arrive = [&]() {
     __builtin_amdgcn_s_waitcnt(vm_wait_imm(0));  // (the compiler does not see the DMA's LDS writes)
     asm volatile("" ::: "memory");
     __syncthreads();
-    if (tile + 1 < tile1) load(tile + 1, nxt);
-    if (live) compute(tile, cur);
-    if (tile + 1 < tile1) store(nxt);
+  };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  // The tiles that count whole for every column go through the stages; the chunk's
+  // others (from `whole` on) one by one.
+  const int whole = ragged ? tile0 : max(tile0, min(tile1, p.tokens / T::kTile));
+  put_k(tile0);
+  put_v(tile0);
+  int tile = tile0;
+  if (tile < whole) {
+    int side = T::kPlane;  // the other planes' distance
+    f32x16 s0, s1;
+    Weights w0, w1;
+    float m;
+    arrive();
+    if (tile + 1 < whole) load_k(tile + 1);
+    if (live) {
+      s0 = scores(0);
+      w0 = stage(yes, no, T::kBlock, 0, s1, s0, w1, m);
+      rescale(m);
+      l_run += w0.sum;
+    }
+    if (tile + 1 < whole) put_k(tile + 1);
+    // Block 1 of `tile`, then block 0 of the next: K of the next tile, V of this one.
+    // (One copy of the loop for both planes: the operands' addresses change sides,
+    // 12 additions a tile, rather than the code.)
+    while (tile + 1 < whole) {
+      arrive();
+      if (tile + 2 < whole) load_k(tile + 2);
+      load_v(tile + 1);
+      if (live) {
+        turn_k(side);
+        w1 = stage(yes, yes, 0, 0, s0, s1, w0, m);
+        rescale(m);
+        l_run += w1.sum;
+        w0 = stage(yes, yes, T::kBlock, T::kBlock, s1, s0, w1, m);
+        rescale(m);
+        l_run += w0.sum;
+        turn_v(side);
+      }
+      if (tile + 2 < whole) put_k(tile + 2);
+      put_v(tile + 1);
+      ++tile;
+      side = -side;
+    }
+    if (tile > tile0) arrive();  // (the last tile's V)
+    if (live) {
+      w1 = stage(no, yes, 0, 0, s0, s1, w0, m);
+      rescale(m);
+      l_run += w1.sum;
+      values(T::kBlock, w1);
+      if (side < 0) {  // (back to the first planes)
+        turn_k(side);
+        turn_v(side);
+      }
+    }
+    ++tile;
+  }
+  for (; tile < tile1; ++tile) {
+    if (tile > tile0) {  // (the first tile is loaded)
+      __syncthreads();
+      load_k(tile);
+      load_v(tile);
+      put_k(tile);
+      put_v(tile);
+    }
+    arrive();
+    if (live) compute_ends(tile);
   }
 
-  // ---- partials
-  const float v_scale = kFp8 ? *p.v_scale : 1.0f;
-  const float l_tot = half_sum(l_run);
-  if (row_ok) {
-    const int64_t idx = ((int64_t)jc * p.Hkv + kvh) * p.rows + row;
-    float* dst = p.part_acc + idx * D + 4 * h;
+  // ---- partials, relative to the maximum itself (the linear sink counts against it)
+  const float to_max = m_max == m_ref ? 1.f : __builtin_amdgcn_exp2f(m_ref - m_max);
+  const float v_scale = (kFp8 ? *p.v_scale : 1.0f) * to_max;
+  const float l_tot = half_sum(l_run) * to_max;
+  const bool none = lim <= first;  // the column ends before this chunk
+  // The accumulators hold a row's sums in 16-byte pieces, 32 rows side by side:
+  // stored like that, each instruction would touch 32 lines for 32 bytes each
+  // (2.4 us of a 29 us kernel).  They go through LDS instead (piece m of row R at
+  // m ^ R, so that neither side meets on a bank), a wave's rows in its own part.
+  constexpr int kPieceRow = D / 4;  // pieces of a row
+  __syncthreads();  // (every wave has done with K and V)
+  const uint32_t mine = lds + wave * (32 * D * 4);
 #pragma unroll
-    for (int d = 0; d < kDb; ++d)
+  for (int d = 0; d < kDb; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *(f32x4*)(dst + 32 * d + 8 * i) = f32x4{acc[d][4 * i] * v_scale, acc[d][4 * i + 1] * v_scale,
-                                                acc[d][4 * i + 2] * v_scale, acc[d][4 * i + 3] * v_scale};
-    if (h == 0) *(f32x2*)(p.part_ml + 2 * idx) = f32x2{m_ref, l_tot};
+    for (int i = 0; i < 4; ++i) {
+      const int m = 8 * d + 2 * i + h;
+      const f32x4 o = none ? f32x4{0.f, 0.f, 0.f, 0.f}
+                           : f32x4{acc[d][4 * i] * v_scale, acc[d][4 * i + 1] * v_scale, acc[d][4 * i + 2] * v_scale,
+                                   acc[d][4 * i + 3] * v_scale};
+      *(lds_f32x4*)(uintptr_t)(mine + (c * kPieceRow + (m ^ (c & (kPieceRow - 1)))) * 16) = o;
+    }
+  const int64_t idx0 = ((int64_t)jc * p.Hkv + kvh) * p.rows + row0;  // the wave's first row
+  if (row_ok && h == 0) *(f32x2*)(p.part_ml + 2 * (idx0 + c)) = none ? f32x2{-INFINITY, 0.f} : f32x2{m_max, l_tot};
+  const int n_pieces = min(32, p.rows - row0) * kPieceRow;  // (<= 0: a wave without rows)
+  float* dst = p.part_acc + idx0 * D;
+#pragma unroll
+  for (int k = 0; k < kPieceRow / 2; ++k) {
+    const int i = k * kWave + lane, R = i / kPieceRow, m = i % kPieceRow;
+    const f32x4 o = *(lds_f32x4*)(uintptr_t)(mine + (R * kPieceRow + (m ^ (R & (kPieceRow - 1)))) * 16);
+    if (i < n_pieces) *(f32x4*)(dst + 4 * i) = o;
+  }
+  if (blockIdx.x == 0) {  // the own parts' lengths, for the kernels that follow
+    for (int i = threadIdx.x; i < p.B; i += 64 * kWaves) p.own_lens[i] = max(clampi(p.lens[i], 0, p.max_len) - p.tokens, 0);
   }
 }
 
@@ -398,9 +628,10 @@ PrefixPlan plan_prefix(int64_t rows, int Hkv, int D, int64_t tokens, int cus) {
   PrefixPlan pl;
   pl.waves = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
   pl.row_tiles = (int)cdiv(rows, 32 * pl.waves);
-  pl.tiles = (int)cdiv(tokens, D <= 128 ? 64 : 32);
-  // workgroups that fit the chip at once: by LDS two of 64 KB a CU (head_dim 64: four of 32 KB)
-  const int64_t slots = (int64_t)cus * (D == 64 ? 4 : 2);
+  pl.tiles = (int)cdiv(tokens, 64);
+  // One workgroup a CU, two where each would have 24 tiles or more: with few tiles
+  // the partials' way to memory and back costs more than the second wave a SIMD gives.
+  const int64_t slots = (int64_t)cus * ((int64_t)pl.tiles * Hkv * pl.row_tiles >= 24 * (int64_t)cus && D <= 128 ? 2 : 1);
   const int64_t want = std::max<int64_t>(1, slots / ((int64_t)Hkv * pl.row_tiles));
   pl.chunk = (int)cdiv(pl.tiles, std::min<int64_t>(want, pl.tiles));
   pl.chunks = (int)cdiv(pl.tiles, pl.chunk);
@@ -416,10 +647,8 @@ struct SharedParts {
 
 template <int D, bool kQBf16, bool kVBf16, bool kFp8>
 int launch_prefix_waves(const PrefixParams& p, int waves, unsigned grid, const Launch& s) {
-  using T = PrefixTile<D>;
-  constexpr uint32_t lds = 4 * T::kPlane;
   auto go = [&](auto kernel) {
-    launch(kernel, dim3(grid), dim3(64 * waves), lds, s, p);
+    launch(kernel, dim3(grid), dim3(64 * waves), 4 * PrefixTile<D>::kPlane, s, p);
     return FSK_OK;
   };
   if (waves == 1) return go(prefix_kernel<D, kQBf16, kVBf16, kFp8, 1>);

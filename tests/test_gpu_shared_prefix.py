@@ -183,6 +183,16 @@ def test_large_scores_and_late_maxima():
     check(batch, batch.run(), "growing scores")
 
 
+def test_linear_sink_counts_against_the_true_maximum():
+    """Maxima that grow within the lazy maximum's 2^8, and sinks that show it."""
+    batch = Batch([1030] * 5, 1024, (32, 8, 128), "f16", seed=20, sinks=True)
+    order = batch.table[0, :64].long()
+    for i in range(64):
+        batch.k[order[i]] *= 0.2 + 0.01 * i
+    batch.sinks.uniform_(20, 60)
+    check(batch, batch.run(sink_mode="linear"), "linear sinks", None, "linear")
+
+
 def test_prefix_of_nothing_and_of_everything():
     batch = Batch([33, 20, 7], 0, (32, 8, 128), "f16", seed=9)
     for shared in (0, 15):  # less than a page: the paged decode itself
