@@ -106,7 +106,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRsrcWord3 = 0x00020000;
 constexpr float E4M3_MAX_F = 448.f;  // largest finite e4m3fn value
 
-enum Layout { kVarlen = 0, kPaged = 1, kDense = 2 };
+// kPagedOwn: the paged layout's tokens past a shared prefix (Params::own_from).
+enum Layout { kVarlen = 0, kPaged = 1, kDense = 2, kPagedOwn = 3 };
+constexpr bool is_paged(int layout) { return layout == kPaged || layout == kPagedOwn; }
 enum Kind { kF16 = FSK_F16, kBF16 = FSK_BF16, kF32 = FSK_F32, kE4M3 = FSK_E4M3 };
 // Q, K and V read as 16-bit values and quantised to e4m3 on the way to the
 // matrix cores (the HF attention function's fp8 form): kQuant + the type.
@@ -387,6 +389,9 @@ struct Params {
   // (amax_n entries each, one tensor after the other).
   const uint32_t* amax;
   int amax_n[3];
+  // kPagedOwn: the tokens before each sequence's own (block_table starts past
+  // them), and the longest whole length.
+  int own_from, whole_max;
 };
 
 // A plan built on the host (the host-plan entry points, for callers that
@@ -416,6 +421,9 @@ __device__ __forceinline__ void seq_range(const Params& p, int b, int& start, in
   } else if constexpr (kLayout == kPaged) {
     start = 0;
     len = clampi(p.lens[b], 0, p.max_blocks * p.page_size);
+  } else if constexpr (kLayout == kPagedOwn) {
+    start = 0;
+    len = max(clampi(p.lens[b], 0, p.whole_max) - p.own_from, 0);
   } else {
     int e = clampi(p.lens[b], 0, p.kv_extent);
     int s = p.starts ? clampi(p.starts[b], 0, e) : 0;
@@ -460,6 +468,11 @@ __device__ __forceinline__ HalfTile half_tile(const Params& p, int b, int start,
   }
   return h;
 }
+
+// A wave of the persistent grid: its lane, its number and how many there are.
+struct Worker {
+  int lane, id, count;
+};
 
 // Work plan.  The sequences' tokens are laid end to end, each sequence padded
 // to a multiple of kAlign (32 tokens, 128 with block scores), and the stream
@@ -633,6 +646,9 @@ __device__ __forceinline__ void seq_range_first(const Params& p, int lane, int& 
   } else if constexpr (kLayout == kPaged) {
     start = 0;
     len = clampi(l0, 0, p.max_blocks * p.page_size);
+  } else if constexpr (kLayout == kPagedOwn) {
+    start = 0;
+    len = max(clampi(l0, 0, p.whole_max) - p.own_from, 0);
   } else {
     const int e = clampi(l0, 0, p.kv_extent);
     start = p.starts ? clampi(s0, 0, e) : 0;
@@ -644,10 +660,10 @@ __device__ __forceinline__ void seq_range_first(const Params& p, int lane, int& 
 // len0: length of sequence `lane` (0 past B), from seq_range_first, whose
 // loads the caller issues first.
 template <int kLayout, bool kScores>
-__device__ __forceinline__ Split build_plan(const Params& p, int32_t* pre, int32_t* flat, const int len0,
+__device__ __forceinline__ Split build_plan(const Params& p, const Worker wk, int32_t* pre, int32_t* flat, const int len0,
                                             int& seg_out, int& flat0_out, int& pre0_out) {
   constexpr int kAlign = kScores ? 128 : 32;
-  const int lane = threadIdx.x;
+  const int lane = wk.lane;
   // Lengths of sequences lane, lane + 64, ...; the first block stays in a
   // register so that the common case (B <= 64) reads them once (and the
   // work loop reads them from these registers, not from memory).
@@ -734,7 +750,7 @@ __device__ __forceinline__ Split build_plan(const Params& p, int32_t* pre, int32
       pre0_out = pb;
     }
     if constexpr (kScores)
-      if (blockIdx.x == 0 && b < p.B) p.lens_out[b] = len;
+      if (wk.id == 0 && b < p.B) p.lens_out[b] = len;
     carry_f += __builtin_amdgcn_readlane(incl_f, kWave - 1);
     carry_u += __builtin_amdgcn_readlane(incl_u, kWave - 1);
   }
@@ -743,7 +759,7 @@ __device__ __forceinline__ Split build_plan(const Params& p, int32_t* pre, int32
     pre[p.B] = min(carry_u, p.u_max);
   }
   __syncthreads();
-  if (blockIdx.x == 0) {
+  if (wk.id == 0) {
     for (int b = lane; b <= p.B; b += kWave) p.plan[b] = pre[b];
   }
   return sp;
@@ -867,7 +883,7 @@ template <int kLayout>
 __device__ __forceinline__ HalfTile unit_half(const Params& p, const Unit& un, int t) {
   HalfTile h;
   h.rows = uniform(clampi(un.t_end - t, 0, 16));
-  if constexpr (kLayout == kPaged) {
+  if constexpr (is_paged(kLayout)) {
     int page = 0, off = 0;
     if (h.rows > 0) {
       const int lp = (int)fdiv((uint32_t)t, p.page);
@@ -900,7 +916,7 @@ __device__ __forceinline__ HalfTile unit_half(const Params& p, const Unit& un, i
 // do block scores (the running block maximum is stored when a block ends).
 template <int kLayout, bool kScores>
 __device__ __forceinline__ int tile_rotation(int kvh, int n_tiles, FastDiv hkv) {
-  if constexpr (kScores || kLayout == kPaged) return 0;
+  if constexpr (kScores || is_paged(kLayout)) return 0;
   return (int)fdiv((uint32_t)(kvh * n_tiles), hkv);  // kvh < Hkv, n_tiles <= 128
 }
 
@@ -1315,22 +1331,17 @@ constexpr int kWavesPerEu = FSK_PIPE_DEPTH > 2 ? 1 : 2;
 __device__ __forceinline__ const HostPlan* plan_ptr() { return nullptr; }
 __device__ __forceinline__ const HostPlan* plan_ptr(const HostPlan& h) { return &h; }
 
-// The partial kernel.  Plan: none (the kernel builds the plan on the device
-// from the lengths) or a HostPlan (built by the host from host lengths,
-// B <= kHostPlanMax; lens_arg and starts_arg are then unused).
-template <int D, int kQ, int kKV, int kLayout, bool kScores, bool kValu = false, typename... Plan>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kWavesPerEu))) void partial_kernel(
-    const int32_t* lens_arg, const int32_t* starts_arg, int B_arg, Params pk, Plan... host_plan) {
-  // The plan's first loads (the lengths) need only these three, which lead
-  // the argument list so that the dispatch preloads them into SGPRs
-  // (-amdgpu-kernarg-preload-count): the length loads issue without waiting
-  // for a kernel-argument load.
-  Params p = pk;
-  p.lens = lens_arg;
-  p.starts = starts_arg;
-  p.B = B_arg;
-  constexpr bool kHostPlan = sizeof...(Plan) == 1;
-  const HostPlan* hp = plan_ptr(host_plan...);
+// The partial kernel's work for one wave.  Plan: hp null (the wave builds the plan
+// on the device from the lengths) or a HostPlan (built by the host from host
+// lengths, B <= kHostPlanMax).  s_kstage: LDS offset of the wave's K stage
+// (partial_stage bytes); s_plan: the wave's plan tables, 2 (B + 1) entries.
+template <int D, int kKV>
+constexpr int partial_stage() {
+  return ((D <= 128) ? FSK_PIPE_DEPTH : 1) * 2 * TileRegs<D, kKV>::kHalfBytes;
+}
+template <int D, int kQ, int kKV, int kLayout, bool kScores, bool kValu, bool kHostPlan>
+__device__ __forceinline__ void partial_work(const Params& p, const HostPlan* hp, const Worker wk,
+                                             const uint32_t s_kstage, int32_t* s_plan) {
   using TR = TileRegs<D, kKV>;
   using SM = Softmax<D, kQ, kKV>;
   constexpr bool kKvFp8 = TR::kFp8;
@@ -1344,13 +1355,9 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kWavesPerEu)
                 "the VALU tile is built for f16, D = 128, paged and varlen");
   static_assert(!kHostPlan || (!kScores && !kValu), "host plans are for the plain decode kernels");
 
-  __shared__ __attribute__((aligned(16))) uint8_t s_kstage_mem[kDepth * 2 * TR::kHalfBytes];
-  // LDS offset of the stage = low 32 bits of its generic address
-  const uint32_t s_kstage = (uint32_t)(uintptr_t)s_kstage_mem;
-  extern __shared__ int32_t s_plan[];
   int32_t* s_pre = s_plan;              // [B+1] first partial of each sequence
   int32_t* s_flat = s_plan + p.B + 1;   // [B+1] stream offset of each sequence
-  const int lane = threadIdx.x;
+  const int lane = wk.lane;
   const int g = lane >> 4;
   const int c = lane & 15;
 
@@ -1393,12 +1400,12 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kWavesPerEu)
   if constexpr (kHostPlan) {
     // Workgroup 0 publishes the unit prefix for the reduce kernel, as
     // build_plan does (lanes past B hold pre[B]).
-    if (blockIdx.x == 0) {
+    if (wk.id == 0) {
       if (lane < p.B) p.plan[lane] = lane_pre;
       if (lane == 0) p.plan[p.B] = hp->pre_end;
     }
   } else {
-    sp = build_plan<kLayout, kScores>(p, s_pre, s_flat, lane_len, seg_x, lane_flat, lane_pre);
+    sp = build_plan<kLayout, kScores>(p, wk, s_pre, s_flat, lane_len, seg_x, lane_flat, lane_pre);
   }
   Requant<kKV> rq;
   amax_scales<kKV>(am, rq);
@@ -1424,7 +1431,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kWavesPerEu)
   const bool pair = (kLayout == kVarlen && D == 128 && !kScores && !kValu) ? (uniform(p.pair) != 0) : false;
   const float sscale = p.score_scale * k_scale;
 
-  for (int w = blockIdx.x; w < W; w += gridDim.x) {
+  for (int w = wk.id; w < W; w += wk.count) {
     int jc, hh;
     item_of(sp, (uint32_t)w, p.nh_div, jc, hh);
     const int kvh = (int)fdiv((uint32_t)hh, p.hb_div);  // (with pair: the pair index, n_hb = 1)
@@ -1457,7 +1464,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kWavesPerEu)
     un.win0 = un.win1 = un.win2 = un.win3 = 0;
     int win_raw0 = 0, win_raw1 = 0, win_raw2 = 0, win_raw3 = 0;
     if (segments_done == 0) FSK_STAMP(8);
-    if constexpr (kLayout == kPaged) {
+    if constexpr (is_paged(kLayout)) {
       un.p_first = (int)fdiv((uint32_t)un.t_begin, p.page);
       const int npg = (int)fdiv((uint32_t)(un.t_end - 1), p.page) - un.p_first + 1;  // <= 256 (chunk <= 4096)
       const int32_t* row = p.block_table + (int64_t)un.b * p.bt_sb + un.p_first;
@@ -1510,7 +1517,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kWavesPerEu)
         qv[h] = h < p.G ? x : u32x4{0, 0, 0, 0};
       }
     }
-    if constexpr (kLayout == kPaged) {
+    if constexpr (is_paged(kLayout)) {
       un.win0 = clampi(win_raw0, 0, p.num_pages - 1);
       un.win1 = clampi(win_raw1, 0, p.num_pages - 1);
       un.win2 = clampi(win_raw2, 0, p.num_pages - 1);
@@ -1645,6 +1652,27 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kWavesPerEu)
   FSK_STAMP(4);
   (void)segments_done;
   (void)hp;
+}
+
+// The partial kernel: one wave a workgroup.  Plan: none or a HostPlan (lens_arg
+// and starts_arg are then unused).
+template <int D, int kQ, int kKV, int kLayout, bool kScores, bool kValu = false, typename... Plan>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kWavesPerEu))) void partial_kernel(
+    const int32_t* lens_arg, const int32_t* starts_arg, int B_arg, Params pk, Plan... host_plan) {
+  // The plan's first loads (the lengths) need only these three, which lead
+  // the argument list so that the dispatch preloads them into SGPRs
+  // (-amdgpu-kernarg-preload-count): the length loads issue without waiting
+  // for a kernel-argument load.
+  Params p = pk;
+  p.lens = lens_arg;
+  p.starts = starts_arg;
+  p.B = B_arg;
+  __shared__ __attribute__((aligned(16))) uint8_t s_kstage_mem[partial_stage<D, kKV>()];
+  extern __shared__ int32_t s_plan[];
+  // LDS offset of the stage = low 32 bits of its generic address
+  partial_work<D, kQ, kKV, kLayout, kScores, kValu, sizeof...(Plan) == 1>(
+      p, plan_ptr(host_plan...), Worker{(int)threadIdx.x, (int)blockIdx.x, (int)gridDim.x},
+      (uint32_t)(uintptr_t)s_kstage_mem, s_plan);
 }
 
 // The sink folded into a row's denominator (M: the row's maximum score, log2
@@ -2998,8 +3026,7 @@ struct Common {
   bool no_timing;          // never stamp this call (no event creation: the allocation-free entry)
   const struct QuantPre* pre;  // quantising decode (dense, f16 / bf16): its first launch, or null
   bool lens_on_host;       // lens is host memory: the plan is built here (make_host_plan)
-  const struct SharedParts* shared;  // partials of a shared prefix that the reduce takes in, or null
-  hipEvent_t last;         // stamped by the last launch (a shared decode's timed call), or null
+  const struct SharedPrefix* shared;  // prefix that all sequences share (then bt and max_blocks are those past it), or null
 };
 
 bool aligned(const void* p, int a) { return ((uintptr_t)p % a) == 0; }
@@ -3440,6 +3467,10 @@ int run_decode(const Common& c) {
   p.num_pages = c.num_pages; p.page_size = c.page_size > 0 ? c.page_size : 16;
   p.page = make_fastdiv((uint32_t)p.page_size);
   p.kv_extent = (int)c.kv_extent;
+  if (c.shared) {
+    p.own_from = c.shared->p.tokens;
+    p.whole_max = c.shared->p.max_len;
+  }
   p.q_scale = c.q_scale; p.k_scale = c.k_scale; p.v_scale = c.v_scale;
   p.score_scale = c.sm_scale * kLog2e;
   p.B = c.B; p.Hkv = c.Hkv; p.G = G; p.n_hb = n_hb;
@@ -3470,7 +3501,7 @@ int run_decode(const Common& c) {
     p.lens_out = (int32_t*)(ws + wl.total + align256((int64_t)c.B * c.Hq * c.nblk * 4));
   }
 
-  const bool valu = g_opt.qk_engine == 1;
+  const bool valu = g_opt.qk_engine == 1 && !c.shared;
   if (valu && !(c.D == 128 && c.q_dt == FSK_F16 && c.kv_dt == FSK_F16 && G <= kValuHeads && !c.scores &&
                 c.layout != FSK_LAYOUT_DENSE))
     return fail(FSK_ERR_UNSUPPORTED, "qk_engine 1 (VALU tile) covers f16 q and KV, head_dim 128, at most 4 query "
@@ -3540,7 +3571,15 @@ int run_decode(const Common& c) {
   int rc;
   const bool sc = c.scores != nullptr;
   const Launch lp{c.stream, ev[0], ev[1]};
-  if (c.lens_on_host) {
+  if (c.shared) {
+    // A wave for every unit of the split up to four a CU (the prefix's workgroups
+    // have the rest of it), in workgroups of four, a multiple of 8 of them.
+    const int own = (int)(cdiv(std::min<int64_t>(grid, 4 * (int64_t)cus), 4 * 8) * 8);
+    if (c.D == 64) launch_shared<64>(*c.shared, p, own, c.q_dt, c.kv_dt, lp);
+    else if (c.D == 128) launch_shared<128>(*c.shared, p, own, c.q_dt, c.kv_dt, lp);
+    else launch_shared<256>(*c.shared, p, own, c.q_dt, c.kv_dt, lp);
+    rc = FSK_OK;
+  } else if (c.lens_on_host) {
     if (c.D == 64 && !pair) rc = dispatch_layout_hp<64>(c.layout, p, hp, grid, c.q_dt, c.kv_dt, lp);
     else if (c.D <= 128) rc = dispatch_layout_hp<128>(c.layout, p, hp, grid, c.q_dt, c.kv_dt, lp);
     else rc = dispatch_layout_hp<256>(c.layout, p, hp, grid, c.q_dt, c.kv_dt, lp);
@@ -3556,7 +3595,7 @@ int run_decode(const Common& c) {
   ReduceParams rp;
   memset(&rp, 0, sizeof(rp));
   if (c.shared) {
-    rp.pre_ml = c.shared->ml; rp.pre_acc = c.shared->acc; rp.n_pre = c.shared->n;
+    rp.pre_ml = c.shared->p.part_ml; rp.pre_acc = c.shared->p.part_acc; rp.n_pre = c.shared->chunks;
     rp.pre_rows = c.B * G;
   }
   rp.plan = p.plan; rp.part_ml = p.part_ml; rp.part_acc = p.part_acc;
@@ -3564,7 +3603,7 @@ int run_decode(const Common& c) {
   rp.out = (uint8_t*)c.out; rp.o_sb = c.o_sb * oe; rp.o_sh = c.o_sh * oe;
   rp.Hq = c.Hq; rp.Hkv = c.Hkv; rp.G = G;
   rp.blk_max = p.blk_max; rp.lens = p.lens_out; rp.scores = (uint8_t*)c.scores; rp.nblk = c.nblk;
-  const Launch lr{c.stream, nullptr, c.last ? c.last : ev[2]};
+  const Launch lr{c.stream, nullptr, ev[2]};
   if (c.D == 64) launch_reduce<64>(rp, c.B, c.o_dt, lr);
   else if (c.D == 128) launch_reduce<128>(rp, c.B, c.o_dt, lr);
   else launch_reduce<256>(rp, c.B, c.o_dt, lr);
@@ -3574,68 +3613,57 @@ int run_decode(const Common& c) {
   return FSK_OK;
 }
 
-// Workspace of a shared-prefix decode: the own lengths, the prefix's partials,
-// then the workspace of the decode of the own tokens.
+// Workspace of a shared-prefix decode: the prefix's partials, then the workspace
+// of the decode of the own tokens.
 struct SharedLayout {
-  int64_t ml_off, acc_off, own_off;
+  int64_t acc_off, own_off;
 };
 SharedLayout shared_layout(const PrefixPlan& pl, int B, int Hq, int D) {
   SharedLayout w;
-  w.ml_off = align256(4 * (int64_t)B);
-  w.acc_off = w.ml_off + align256((int64_t)pl.chunks * B * Hq * 2 * 4);
+  w.acc_off = align256((int64_t)pl.chunks * B * Hq * 2 * 4);
   w.own_off = w.acc_off + align256((int64_t)pl.chunks * B * Hq * (int64_t)D * 4);
   return w;
 }
-int64_t own_workspace(int B, int Hq, int Hkv, int D, int own_blocks, int page_size) {
-  return fsk_workspace_bytes(FSK_LAYOUT_PAGED, B, Hq, Hkv, D, own_blocks, page_size, 0);
+// Whole pages that the batch is decoded with as shared (0: as the paged decode).
+int64_t shared_pages(int B, int64_t shared_len, int page_size) {
+  return B == 0 || B > kSharedMaxBatch ? 0 : shared_len / page_size;
 }
 int64_t shared_workspace(int B, int Hq, int Hkv, int D, int64_t max_blocks, int page_size, int64_t shared_len) {
   const int64_t whole = fsk_workspace_bytes(FSK_LAYOUT_PAGED, B, Hq, Hkv, D, max_blocks, page_size, 0);
   if (whole < 0) return whole;
   if (shared_len < 0 || shared_len > max_blocks * page_size)
     return fail(FSK_ERR_INVALID, "shared_len must be in [0, max_blocks * page_size]");
-  const int64_t common = shared_len / page_size;
-  if (common == 0 || B == 0) return whole;
+  const int64_t common = shared_pages(B, shared_len, page_size);
+  if (common == 0) return whole;
   const PrefixPlan pl = plan_prefix((int64_t)B * (Hq / Hkv), Hkv, D, common * page_size, device_cus());
-  const int64_t own = own_workspace(B, Hq, Hkv, D, (int)(max_blocks - common), page_size);
+  const int64_t own = fsk_workspace_bytes(FSK_LAYOUT_PAGED, B, Hq, Hkv, D, max_blocks - common, page_size, 0);
   if (own < 0) return own;
   return shared_layout(pl, B, Hq, D).own_off + own;
 }
 
 // Paged decode whose sequences share their first shared_len tokens' pages:
-// prefix_kernel over the shared pages, the split kernel over each sequence's
-// own (its lengths come from the prefix kernel), and the reduce over both.
+// shared_kernel over the shared pages and each sequence's own, and the reduce
+// over both.
 int run_shared(const Common& c, int64_t shared_len) {
-  int st = validate(c);
+  const int st = validate(c);
   if (st != FSK_OK) return st;
   if (shared_len < 0 || shared_len > (int64_t)c.max_blocks * c.page_size)
     return fail(FSK_ERR_INVALID, "shared_len must be in [0, max_blocks * page_size]");
-  const int common = (int)(shared_len / c.page_size);  // whole shared pages
-  if (c.B == 0 || common == 0) return run_decode(c);
+  const int common = (int)shared_pages(c.B, shared_len, c.page_size);
+  if (common == 0) return run_decode(c);
   const int G = c.Hq / c.Hkv;
   const PrefixPlan pl = plan_prefix((int64_t)c.B * G, c.Hkv, c.D, (int64_t)common * c.page_size, device_cus());
-  const int64_t grid = cdiv((int64_t)pl.chunks * c.Hkv, 8) * 8 * pl.row_tiles;
-  if (grid >= (1 << 24)) return fail(FSK_ERR_UNSUPPORTED, "too many work units");
+  const int64_t blocks = cdiv((int64_t)pl.chunks * c.Hkv, 8) * 8 * pl.row_tiles;
+  if (blocks >= (1 << 23)) return fail(FSK_ERR_UNSUPPORTED, "too many work units");
   const SharedLayout wl = shared_layout(pl, c.B, c.Hq, c.D);
-  const int64_t own_ws = own_workspace(c.B, c.Hq, c.Hkv, c.D, c.max_blocks - common, c.page_size);
-  if (own_ws < 0) return (int)own_ws;
-  if (!c.ws || c.ws_bytes < wl.own_off + own_ws || !aligned(c.ws, 256))
+  if (!c.ws || c.ws_bytes < wl.own_off || !aligned(c.ws, 256))  // (the rest is the decode's to check)
     return fail(FSK_ERR_WORKSPACE, "workspace missing, unaligned or smaller than fsk_shared_workspace_bytes()");
   uint8_t* ws = (uint8_t*)c.ws;
-  const SharedParts parts{(float*)(ws + wl.ml_off), (float*)(ws + wl.acc_off), pl.chunks};
-  Common own = c;
-  own.bt = c.bt + common;
-  own.max_blocks = c.max_blocks - common;
-  own.kv_extent = own.max_blocks;
-  own.lens = (const int32_t*)ws;
-  own.ws = ws + wl.own_off;
-  own.ws_bytes = c.ws_bytes - wl.own_off;
-  own.shared = &parts;
-  own.no_timing = true;
-
   const int qe = elem_bytes(c.q_dt), ke = elem_bytes(c.kv_dt);
-  PrefixParams p;
-  memset(&p, 0, sizeof(p));
+  SharedPrefix sh;
+  memset(&sh, 0, sizeof(sh));
+  sh.chunks = pl.chunks;
+  PrefixParams& p = sh.p;
   p.q = (const uint8_t*)c.q;
   p.q_sb = c.q_sb * qe; p.q_sh = c.q_sh * qe;
   p.k = (const uint8_t*)c.k; p.v = (const uint8_t*)c.v;
@@ -3644,7 +3672,7 @@ int run_shared(const Common& c, int64_t shared_len) {
   p.pages = c.bt;
   p.page = make_fastdiv((uint32_t)c.page_size);
   p.num_pages = c.num_pages;
-  p.lens = c.lens; p.own_lens = (int32_t*)ws;
+  p.lens = c.lens;
   p.max_len = c.max_blocks * c.page_size;
   p.k_scale = c.k_scale; p.v_scale = c.v_scale;
   p.score_scale = c.sm_scale * kLog2e;
@@ -3654,25 +3682,16 @@ int run_shared(const Common& c, int64_t shared_len) {
   p.rt_div = make_fastdiv((uint32_t)pl.row_tiles);
   p.tokens = common * c.page_size; p.tiles = pl.tiles; p.chunk = pl.chunk;
   p.units = pl.chunks * c.Hkv;
-  p.part_ml = (float*)(ws + wl.ml_off); p.part_acc = (float*)(ws + wl.acc_off);
-  (void)hipGetLastError();
-  // Timed calls: the prefix kernel's dispatch stamps its start and end, the
-  // last launch its end.
-  hipEvent_t ev[3] = {nullptr, nullptr, nullptr};
-  if (!c.no_timing) timing_events(ev);
-  const Launch l{c.stream, ev[0], ev[1]};
-  if (c.D == 64) launch_prefix<64>(p, c.q_dt, c.kv_dt, pl.waves, (unsigned)grid, l);
-  else if (c.D == 128) launch_prefix<128>(p, c.q_dt, c.kv_dt, pl.waves, (unsigned)grid, l);
-  else launch_prefix<256>(p, c.q_dt, c.kv_dt, pl.waves, (unsigned)grid, l);
-  const hipError_t e = hipGetLastError();  // (the decode below clears the error state before its launches)
-  if (e != hipSuccess) {
-    timing_keep(ev, false);
-    return fail(FSK_ERR_HIP, std::string("prefix kernel launch failed: ") + hipGetErrorString(e));
-  }
-  own.last = ev[2];
-  st = run_decode(own);
-  timing_keep(ev, st == FSK_OK);
-  return st;
+  p.blocks = (int)blocks;
+  p.part_ml = (float*)ws; p.part_acc = (float*)(ws + wl.acc_off);
+  Common own = c;
+  own.bt = c.bt + common;
+  own.max_blocks = c.max_blocks - common;
+  own.kv_extent = own.max_blocks;
+  own.ws = ws + wl.own_off;
+  own.ws_bytes = c.ws_bytes - wl.own_off;
+  own.shared = &sh;
+  return run_decode(own);
 }
 
 

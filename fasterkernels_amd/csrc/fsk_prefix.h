@@ -23,13 +23,13 @@ struct PrefixParams {
   int num_pages;
   const int32_t* lens;                    // [B] whole lengths
   int max_len;                            // ... clamped to [0, max_len]
-  int32_t* own_lens;                      // [B] out: tokens past the prefix
   const float* k_scale;
   const float* v_scale;
   float score_scale;                      // sm_scale * log2(e)
   int B, G, Hkv, rows;                    // rows: M = B G
   FastDiv g_div, hkv_div, rt_div;         // divisors G, Hkv, row tiles
   int tokens, tiles, chunk;               // shared tokens, their tiles, tiles of a work item
+  int blocks;                             // workgroups of the prefix
   int units;                              // (chunk, KV head) pairs
   float* part_ml;                         // [chunks, Hkv, M, 2]
   float* part_acc;                        // [chunks, Hkv, M, D]
@@ -101,21 +101,20 @@ __device__ __forceinline__ int v_swizzle(int row) {
 // multiplied.  Tile t's K is therefore needed one stage before its V, and their
 // buffers are refilled at different times: with one barrier a tile, K of tile
 // t + 2 and V of tile t + 1 are loaded while blocks 2 t + 1 and 2 t + 2 go through.
-template <int D, bool kQBf16, bool kVBf16, bool kFp8, int kWaves>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(PrefixTile<D>::kPerEu, PrefixTile<D>::kPerEu)))
-void prefix_kernel(PrefixParams p) {
+constexpr int kPrefixWaves = 4;
+template <int D, bool kQBf16, bool kVBf16, bool kFp8>
+__device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_t block, const uint32_t lds) {
   using T = PrefixTile<D>;
+  constexpr int kWaves = kPrefixWaves;
   constexpr int kSteps = D / 16;    // QK k-steps
   constexpr int kDb = D / 32;       // output blocks of 32 dims
-  extern __shared__ __attribute__((aligned(16))) uint8_t s_prefix[];  // K, K, V, V
-  const uint32_t lds = (uint32_t)(uintptr_t)s_prefix;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = uniform((int)threadIdx.x / kWave);
   const int h = lane >> 5, c = lane & 31;
 
   // Row tiles of one (chunk, head) on one XCD, one after the other: they read
   // the same K and V through its L2.
-  const uint32_t xcd = blockIdx.x & 7, in_xcd = blockIdx.x >> 3;
+  const uint32_t xcd = block & 7, in_xcd = block >> 3;
   const uint32_t group = fdiv(in_xcd, p.rt_div);
   const int rt = (int)(in_xcd - group * p.rt_div.d);
   const uint32_t unit = group * 8 + xcd;
@@ -611,23 +610,53 @@ void prefix_kernel(PrefixParams p) {
     const f32x4 o = *(lds_f32x4*)(uintptr_t)(mine + (R * kPieceRow + (m ^ (R & (kPieceRow - 1)))) * 16);
     if (i < n_pieces) *(f32x4*)(dst + 4 * i) = o;
   }
-  if (blockIdx.x == 0) {  // the own parts' lengths, for the kernels that follow
-    for (int i = threadIdx.x; i < p.B; i += 64 * kWaves) p.own_lens[i] = max(clampi(p.lens[i], 0, p.max_len) - p.tokens, 0);
+}
+
+// The whole of a shared decode but the merge: workgroups up to pp.blocks take the
+// prefix, the others the sequences' own tokens (partial_work, a wave each), so
+// that the own tokens' K and V stream in while the matrix cores are busy with
+// the prefix.  Registers and LDS let two workgroups on a CU; the first 256 of
+// each kind share the CUs.  In turn instead (prefix, own tokens, merge) 256 x
+// 4096 + 128 tokens took 34 + 31 us in the first two.
+template <int D, int kKV>
+constexpr uint32_t shared_stage() {
+  constexpr uint32_t prefix = 4 * PrefixTile<D>::kPlane, own = kPrefixWaves * partial_stage<D, kKV>();
+  return prefix > own ? prefix : own;
+}
+template <int D, int kQ, int kKV>
+__global__ __launch_bounds__(64 * kPrefixWaves)
+    __attribute__((amdgpu_waves_per_eu(PrefixTile<D>::kPerEu, PrefixTile<D>::kPerEu)))
+void shared_kernel(const int32_t* lens_arg, const int32_t* starts_arg, int B_arg, PrefixParams pp, Params pk) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_shared[];
+  const uint32_t lds = (uint32_t)(uintptr_t)s_shared;
+  if ((int)blockIdx.x < pp.blocks) {
+    prefix_work<D, kQ == kBF16, kKV == kBF16, kKV == kE4M3>(pp, blockIdx.x, lds);
+    return;
   }
+  Params p = pk;
+  p.lens = lens_arg;
+  p.starts = starts_arg;
+  p.B = B_arg;
+  // (wave w of workgroup b is worker w S + b of 4 S, S a multiple of 8: the
+  // workers' numbers keep to the XCDs as those of one-wave workgroups do)
+  const int b = (int)blockIdx.x - pp.blocks, S = (int)gridDim.x - pp.blocks;
+  const int wave = uniform((int)threadIdx.x / kWave);
+  partial_work<D, kQ, kKV, kPagedOwn, false, false, false>(
+      p, nullptr, Worker{(int)threadIdx.x & (kWave - 1), wave * S + b, kPrefixWaves * S},
+      lds + wave * partial_stage<D, kKV>(), (int32_t*)(s_shared + shared_stage<D, kKV>()) + wave * 2 * (p.B + 1));
 }
 
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-// The prefix's work split: waves of a workgroup, row tiles, tiles of an item and
-// items per KV head (chunks).
+// The prefix's work split: row tiles, tiles of an item and items per KV head
+// (chunks).
 struct PrefixPlan {
-  int waves, row_tiles, tiles, chunk, chunks;
+  int row_tiles, tiles, chunk, chunks;
 };
 PrefixPlan plan_prefix(int64_t rows, int Hkv, int D, int64_t tokens, int cus) {
   PrefixPlan pl;
-  pl.waves = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-  pl.row_tiles = (int)cdiv(rows, 32 * pl.waves);
+  pl.row_tiles = (int)cdiv(rows, 32 * kPrefixWaves);
   pl.tiles = (int)cdiv(tokens, 64);
   // One workgroup a CU, two where each would have 24 tiles or more: with few tiles
   // the partials' way to memory and back costs more than the second wave a SIMD gives.
@@ -637,28 +666,28 @@ PrefixPlan plan_prefix(int64_t rows, int Hkv, int D, int64_t tokens, int cus) {
   pl.chunks = (int)cdiv(pl.tiles, pl.chunk);
   return pl;
 }
+// Sequences whose plan tables, one for each wave, fit LDS beside the tiles (160 KB
+// a CU, 128 KB of tiles at head_dim 256).
+constexpr int kSharedMaxBatch = 1000;
+constexpr uint32_t shared_tables(int B) { return kPrefixWaves * 8 * (uint32_t)(B + 1); }
+static_assert(shared_stage<256, kF16>() + shared_tables(kSharedMaxBatch) <= 160 * 1024, "tiles and tables fit LDS");
 
-// The prefix partials that a decode's reduce kernel takes in.
-struct SharedParts {
-  const float* ml;
-  const float* acc;
-  int n;
+// The shared prefix of a decode (run_shared): the kernel's parameters and the
+// prefix partials that the reduce kernel takes in.
+struct SharedPrefix {
+  PrefixParams p;
+  int chunks;
 };
 
-template <int D, bool kQBf16, bool kVBf16, bool kFp8>
-int launch_prefix_waves(const PrefixParams& p, int waves, unsigned grid, const Launch& s) {
-  auto go = [&](auto kernel) {
-    launch(kernel, dim3(grid), dim3(64 * waves), 4 * PrefixTile<D>::kPlane, s, p);
-    return FSK_OK;
-  };
-  if (waves == 1) return go(prefix_kernel<D, kQBf16, kVBf16, kFp8, 1>);
-  if (waves == 2) return go(prefix_kernel<D, kQBf16, kVBf16, kFp8, 2>);
-  return go(prefix_kernel<D, kQBf16, kVBf16, kFp8, 4>);
+template <int D, int kQ, int kKV>
+void launch_shared_as(const SharedPrefix& sh, const Params& p, int own_blocks, const Launch& s) {
+  launch(shared_kernel<D, kQ, kKV>, dim3((unsigned)(sh.p.blocks + own_blocks)), dim3(64 * kPrefixWaves),
+         shared_stage<D, kKV>() + shared_tables(p.B), s, p.lens, p.starts, p.B, sh.p, p);
 }
 template <int D>
-int launch_prefix(const PrefixParams& p, int q_dt, int kv_dt, int waves, unsigned grid, const Launch& s) {
-  if (kv_dt == FSK_F16) return launch_prefix_waves<D, false, false, false>(p, waves, grid, s);
-  if (kv_dt == FSK_BF16) return launch_prefix_waves<D, true, true, false>(p, waves, grid, s);
-  if (q_dt == FSK_F16) return launch_prefix_waves<D, false, false, true>(p, waves, grid, s);
-  return launch_prefix_waves<D, true, false, true>(p, waves, grid, s);
+void launch_shared(const SharedPrefix& sh, const Params& p, int own_blocks, int q_dt, int kv_dt, const Launch& s) {
+  if (kv_dt == FSK_F16) launch_shared_as<D, kF16, kF16>(sh, p, own_blocks, s);
+  else if (kv_dt == FSK_BF16) launch_shared_as<D, kBF16, kBF16>(sh, p, own_blocks, s);
+  else if (q_dt == FSK_F16) launch_shared_as<D, kF16, kE4M3>(sh, p, own_blocks, s);
+  else launch_shared_as<D, kBF16, kE4M3>(sh, p, own_blocks, s);
 }
