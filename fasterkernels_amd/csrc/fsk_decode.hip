@@ -1870,9 +1870,9 @@ __device__ __forceinline__ void reduce_rows(const ReduceParams& p, int h0, int b
 }
 
 // One workgroup per (query head, sequence).
-template <int D, int kOut, bool kShared>
+template <int D, int kOut>
 __global__ __launch_bounds__(kReduceThreads) void reduce_kernel(ReduceParams p) {
-  reduce_rows<D, kOut, 1, kShared>(p, blockIdx.x, blockIdx.y, threadIdx.x);
+  reduce_rows<D, kOut, 1, false>(p, blockIdx.x, blockIdx.y, threadIdx.x);
 }
 
 // For many rows (more than the 2048 workgroups that fit the chip at once),
@@ -1896,7 +1896,7 @@ __global__ __launch_bounds__(kReduceThreads) void reduce_kernel(ReduceParams p) 
 constexpr int kFewUnits = 16;    // partials of a sequence that count as few
 constexpr int kLongGroups = 256;
 template <int D, int kOut, int kManyRows, bool kShared>
-__global__ __launch_bounds__(kReduceThreads) void reduce_many_kernel(ReduceParams p, int B, FastDiv per_seq) {
+__device__ __forceinline__ void reduce_many(const ReduceParams& p, int B, FastDiv per_seq) {
   if ((int)blockIdx.x >= kLongGroups) {
     const uint32_t i = blockIdx.x - kLongGroups;
     const uint32_t b = fdiv(i, per_seq);  // per_seq = Hq / kManyRows workgroups of a sequence
@@ -1945,6 +1945,21 @@ __global__ __launch_bounds__(kReduceThreads) void reduce_many_kernel(ReduceParam
     before += here;
     __syncthreads();
   }
+}
+
+template <int D, int kOut, int kManyRows>
+__global__ __launch_bounds__(kReduceThreads) void reduce_many_kernel(ReduceParams p, int B, FastDiv per_seq) {
+  reduce_many<D, kOut, kManyRows, false>(p, B, per_seq);
+}
+
+// The same with the partials of a shared prefix beside each sequence's own.
+template <int D, int kOut>
+__global__ __launch_bounds__(kReduceThreads) void shared_reduce_kernel(ReduceParams p) {
+  reduce_rows<D, kOut, 1, true>(p, blockIdx.x, blockIdx.y, threadIdx.x);
+}
+template <int D, int kOut, int kManyRows>
+__global__ __launch_bounds__(kReduceThreads) void shared_reduce_many_kernel(ReduceParams p, int B, FastDiv per_seq) {
+  reduce_many<D, kOut, kManyRows, true>(p, B, per_seq);
 }
 
 // ---------------------------------------------------------------------------
@@ -2824,6 +2839,7 @@ struct Options {
   int head_pairs = 1;           // varlen, head_dim 64: neighbouring KV heads as one 128-wide row (see pair_shape)
   int seg_tokens = 96;          // lead-in per sequence in the work stream where boundaries are common (tokens)
   int direct = 1;               // calls of short sequences on the direct kernel (see direct_waves); 0: never
+  int share = 1;                // shared prefixes: 1 where it pays (see shared_pays), 0 never, 2 always
 } g_opt;
 
 // Event triples of timed decode calls (the partial kernel's start and end and
@@ -3191,21 +3207,24 @@ FastDiv make_fastdiv(uint32_t d) {
   return FastDiv{d, (uint32_t)((two_s + d - 1) / d), 31 + l};
 }
 
-template <int D, int kOut, bool kShared>
+template <int D, int kOut>
 void launch_reduce_out(const ReduceParams& rp, int B, int rows, const Launch& s) {
+  const bool shared = rp.n_pre > 0;
   if (rows == 1) {
-    launch(reduce_kernel<D, kOut, kShared>, dim3(rp.Hq, B), dim3(kReduceThreads), 0, s, rp);
+    launch(shared ? shared_reduce_kernel<D, kOut> : reduce_kernel<D, kOut>, dim3(rp.Hq, B), dim3(kReduceThreads), 0, s, rp);
     return;
   }
   const dim3 grid((unsigned)(kLongGroups + (int64_t)rp.Hq / rows * B));
   const FastDiv per_seq = make_fastdiv((uint32_t)(rp.Hq / rows));
   if constexpr (D <= 128) {
     if (rows == 8) {
-      launch(reduce_many_kernel<D, kOut, 8, kShared>, grid, dim3(kReduceThreads), 0, s, rp, B, per_seq);
+      launch(shared ? shared_reduce_many_kernel<D, kOut, 8> : reduce_many_kernel<D, kOut, 8>, grid, dim3(kReduceThreads),
+             0, s, rp, B, per_seq);
       return;
     }
   }
-  launch(reduce_many_kernel<D, kOut, 4, kShared>, grid, dim3(kReduceThreads), 0, s, rp, B, per_seq);
+  launch(shared ? shared_reduce_many_kernel<D, kOut, 4> : reduce_many_kernel<D, kOut, 4>, grid, dim3(kReduceThreads), 0,
+         s, rp, B, per_seq);
 }
 
 // More rows than workgroups fit at once (2048 of 256 threads on 256 CUs): see
@@ -3219,14 +3238,9 @@ void launch_reduce(const ReduceParams& rp, int B, int o_dt, const Launch& s) {
   const int64_t total = (int64_t)rp.Hq * B;
   int rows = D <= 128 && rp.Hq % 8 == 0 ? 8 : rp.Hq % 4 == 0 ? 4 : 1;
   if (total <= 2048 || total / rows + kLongGroups >= (1 << 24) || rp.scores) rows = 1;
-  auto out = [&](auto shared) {
-    constexpr bool kShared = decltype(shared)::value;
-    if (o_dt == FSK_F16) launch_reduce_out<D, kF16, kShared>(rp, B, rows, s);
-    else if (o_dt == FSK_BF16) launch_reduce_out<D, kBF16, kShared>(rp, B, rows, s);
-    else launch_reduce_out<D, kF32, kShared>(rp, B, rows, s);
-  };
-  if (rp.n_pre > 0) out(std::true_type{});
-  else out(std::false_type{});
+  if (o_dt == FSK_F16) launch_reduce_out<D, kF16>(rp, B, rows, s);
+  else if (o_dt == FSK_BF16) launch_reduce_out<D, kBF16>(rp, B, rows, s);
+  else launch_reduce_out<D, kF32>(rp, B, rows, s);
 }
 
 // The split policy's per-call constants (see SplitArgs): target_units <=
@@ -3572,9 +3586,10 @@ int run_decode(const Common& c) {
   const bool sc = c.scores != nullptr;
   const Launch lp{c.stream, ev[0], ev[1]};
   if (c.shared) {
-    // A wave for every unit of the split up to four a CU (the prefix's workgroups
-    // have the rest of it), in workgroups of four, a multiple of 8 of them.
-    const int own = (int)(cdiv(std::min<int64_t>(grid, 4 * (int64_t)cus), 4 * 8) * 8);
+    // A wave for every unit of the split in up to a workgroup a CU (the prefix's have
+    // the rest of it), a multiple of 8 of them; at head_dim 256 with eight waves
+    // each, of which the first four take what there is on all CUs.
+    const int own = (int)(cdiv(std::min<int64_t>(cdiv(grid, 4), cus), 8) * 8);
     if (c.D == 64) launch_shared<64>(*c.shared, p, own, c.q_dt, c.kv_dt, lp);
     else if (c.D == 128) launch_shared<128>(*c.shared, p, own, c.q_dt, c.kv_dt, lp);
     else launch_shared<256>(*c.shared, p, own, c.q_dt, c.kv_dt, lp);
@@ -3624,9 +3639,26 @@ SharedLayout shared_layout(const PrefixPlan& pl, int B, int Hq, int D) {
   w.own_off = w.acc_off + align256((int64_t)pl.chunks * B * Hq * (int64_t)D * 4);
   return w;
 }
-// Whole pages that the batch is decoded with as shared (0: as the paged decode).
+// Whole pages that a batch can be decoded with as shared (0: as the paged decode).
 int64_t shared_pages(int B, int64_t shared_len, int page_size) {
   return B == 0 || B > kSharedMaxBatch ? 0 : shared_len / page_size;
+}
+// Whether sharing pays: a call that the direct kernel would take is faster left to
+// it (32 heads on 8 x 128 fp16, 512 tokens shared by 8, 32, 64 sequences: 10.5,
+// 9.7, 12.1 us, shared 10.6, 13.4, 16.9), and the split kernels re-read a short
+// prefix from cache faster than the prefix's partials are merged, below 32 MB of
+// K/V re-reads (1024 tokens, 4, 8, 16, 64 sequences, 17 to 268 MB: 11.7, 13.2, 13.6,
+// 27.7 us, shared 11.9, 11.9, 13.2, 22.3; 64 heads on 8 x 64, 2048 tokens, 4, 8,
+// 32: 12.1, 13.8, 22.8, shared 11.1, 12.7, 16.8).  At head_dim 256, where one
+// workgroup fills a CU, below 64 MB, 256 MB for bf16 with its two products a weight
+// (fp16 4096 tokens, 4, 8, 16 sequences: 25.2, 38.0, 58.8, shared 28.0, 31.6, 35.7;
+// bf16 24.8, 38.4, 59.4, shared 36.0, 37.6, 41.5).
+bool shared_pays(const Common& c, int64_t common) {
+  if (g_opt.share != 1) return g_opt.share == 2;
+  if (direct_waves(c, (int64_t)c.B * plan_heads(c.layout, c.D, c.Hkv, c.Hq / c.Hkv), false)) return false;
+  const int64_t reads = c.B * common * c.page_size * 2 * c.Hkv * c.D * elem_bytes(c.kv_dt);
+  const int64_t least = c.D <= 128 ? 32 : c.kv_dt == FSK_BF16 ? 256 : 64;
+  return reads >= least * 1000000;
 }
 int64_t shared_workspace(int B, int Hq, int Hkv, int D, int64_t max_blocks, int page_size, int64_t shared_len) {
   const int64_t whole = fsk_workspace_bytes(FSK_LAYOUT_PAGED, B, Hq, Hkv, D, max_blocks, page_size, 0);
@@ -3638,7 +3670,7 @@ int64_t shared_workspace(int B, int Hq, int Hkv, int D, int64_t max_blocks, int 
   const PrefixPlan pl = plan_prefix((int64_t)B * (Hq / Hkv), Hkv, D, common * page_size, device_cus());
   const int64_t own = fsk_workspace_bytes(FSK_LAYOUT_PAGED, B, Hq, Hkv, D, max_blocks - common, page_size, 0);
   if (own < 0) return own;
-  return shared_layout(pl, B, Hq, D).own_off + own;
+  return std::max(whole, shared_layout(pl, B, Hq, D).own_off + own);
 }
 
 // Paged decode whose sequences share their first shared_len tokens' pages:
@@ -3650,7 +3682,7 @@ int run_shared(const Common& c, int64_t shared_len) {
   if (shared_len < 0 || shared_len > (int64_t)c.max_blocks * c.page_size)
     return fail(FSK_ERR_INVALID, "shared_len must be in [0, max_blocks * page_size]");
   const int common = (int)shared_pages(c.B, shared_len, c.page_size);
-  if (common == 0) return run_decode(c);
+  if (common == 0 || !shared_pays(c, common)) return run_decode(c);
   const int G = c.Hq / c.Hkv;
   const PrefixPlan pl = plan_prefix((int64_t)c.B * G, c.Hkv, c.D, (int64_t)common * c.page_size, device_cus());
   const int64_t blocks = cdiv((int64_t)pl.chunks * c.Hkv, 8) * 8 * pl.row_tiles;
@@ -3946,6 +3978,11 @@ int fsk_set_option(const char* name, int64_t value) {
   if (!strcmp(name, "chunk_tokens")) {
     if (value < 0 || value % 32 || value > (1 << 20)) return fail(FSK_ERR_INVALID, "chunk_tokens: 0 or a multiple of 32");
     g_opt.chunk_tokens = (int)value;
+    return FSK_OK;
+  }
+  if (!strcmp(name, "share")) {
+    if (value < 0 || value > 2) return fail(FSK_ERR_INVALID, "share: 0, 1 or 2");
+    g_opt.share = (int)value;
     return FSK_OK;
   }
   if (!strcmp(name, "seg_tokens")) {

@@ -75,8 +75,12 @@ struct PrefixTile {
   static constexpr int kChunks = kRow / 16;
   static constexpr int kPlane = kTile * kRow;    // one tile of K or V
   static constexpr int kBlock = 32 * kRow;       // a score block's rows
-  static constexpr int kHalves = kTile / 16;     // 16-token pieces, each inside one page
-  static constexpr int kPerEu = D <= 128 ? 2 : 1;  // waves a SIMD the registers are sized for
+  static constexpr int kPieces = kTile / 16;     // 16-token pieces, each inside one page
+  // Waves of a workgroup: four of 32 query rows; at head_dim 256 four pairs, each
+  // wave of a pair with half of the output dims (and all of the products: their
+  // sums and Q together are too many registers for one wave of a SIMD's two).
+  static constexpr int kSplit = D <= 128 ? 1 : 2;
+  static constexpr int kWaves = 4 * kSplit;
 };
 // V chunk m of row R is stored at m ^ v_swizzle(R): a transposing read takes 4
 // rows x 64 bytes a half-wave, which land on different banks (64 of 4 bytes).
@@ -101,15 +105,15 @@ __device__ __forceinline__ int v_swizzle(int row) {
 // multiplied.  Tile t's K is therefore needed one stage before its V, and their
 // buffers are refilled at different times: with one barrier a tile, K of tile
 // t + 2 and V of tile t + 1 are loaded while blocks 2 t + 1 and 2 t + 2 go through.
-constexpr int kPrefixWaves = 4;
 template <int D, bool kQBf16, bool kVBf16, bool kFp8>
 __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_t block, const uint32_t lds) {
   using T = PrefixTile<D>;
-  constexpr int kWaves = kPrefixWaves;
+  constexpr int kRows = 128;        // query rows of a workgroup
   constexpr int kSteps = D / 16;    // QK k-steps
-  constexpr int kDb = D / 32;       // output blocks of 32 dims
+  constexpr int kDb = D / 32 / T::kSplit;  // the wave's output blocks of 32 dims
   const int lane = threadIdx.x & (kWave - 1);
-  const int wave = uniform((int)threadIdx.x / kWave);
+  const int wave_id = uniform((int)threadIdx.x / kWave);
+  const int wave = wave_id & 3, part = wave_id >> 2;  // 32 rows, and with kSplit a half of the dims
   const int h = lane >> 5, c = lane & 31;
 
   // Row tiles of one (chunk, head) on one XCD, one after the other: they read
@@ -125,15 +129,14 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
 
   // ---- first loads, in flight together: the pages of the wave's first 64
   // 16-token pieces (lane i: piece base + i), the query rows and the lengths.
-  // The wave stages pieces wave, wave + kWaves, .. of a tile.
-  constexpr int kPieces = T::kHalves / kWaves;
-  int win_base = tile0 * T::kHalves;
+  // The wave stages piece `wave` of every tile (with kSplit K or V of it).
+  int win_base = tile0 * T::kPieces;
   auto page_of = [&](int piece) {
     const int t = min(16 * piece, p.tokens - 1);  // (pieces past the prefix are not staged)
     return p.pages[fdiv((uint32_t)t, p.page)];
   };
   const int first_page = page_of(win_base + lane);
-  const int row0 = (rt * kWaves + wave) * 32;
+  const int row0 = rt * kRows + wave * 32;
   const bool live = row0 < p.rows;                // any column of the wave is a query row
   const int row = min(row0 + c, p.rows - 1);
   const bool row_ok = row0 + c < p.rows;
@@ -163,40 +166,42 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
   // 1 KB = 1024 / D rows, kept in registers until the buffer is free.
   constexpr int kDma = 16 * T::kRow / 1024;
   constexpr int kCodeLoads = 16 * D / 1024;
-  constexpr int kCodes = kFp8 ? kPieces * kCodeLoads : 1;
+  constexpr int kCodes = kFp8 ? kCodeLoads : 1;
   u32x4 k_codes[kCodes], v_codes[kCodes];
-  int k_off[kDma], v_off[kDma];
-  if constexpr (!kFp8) {
+  // Byte offsets of the lane's 16 bytes in DMA load r of a piece, kept in registers
+  // but at head_dim 256, which has none to spare.
+  auto dma_off = [&](auto is_v, int r) {
+    constexpr bool kV = decltype(is_v)::value;
+    const int R = r * (64 / T::kChunks) + lane / T::kChunks, m = lane % T::kChunks;
+    return R * (int)(kV ? p.v_st : p.k_st) + 16 * (m ^ (kV ? v_swizzle<T::kChunks>(R) : k_swizzle<T::kChunks>(R)));
+  };
+  constexpr int kOffs = D <= 128 ? kDma : 1;
+  int k_off[kOffs], v_off[kOffs];
+  if constexpr (!kFp8 && D <= 128) {
 #pragma unroll
     for (int r = 0; r < kDma; ++r) {
-      const int R = r * (64 / T::kChunks) + lane / T::kChunks;
-      const int m = lane % T::kChunks;
-      k_off[r] = R * (int)p.k_st + 16 * (m ^ k_swizzle<T::kChunks>(R));
-      v_off[r] = R * (int)p.v_st + 16 * (m ^ v_swizzle<T::kChunks>(R));
+      k_off[r] = dma_off(std::false_type{}, r);
+      v_off[r] = dma_off(std::true_type{}, r);
     }
   }
   // This wave's pieces of a tile's K or V into a plane (16-bit), or into registers
   // (e4m3) from which put() widens them into it.  Pieces past the prefix read as zeros.
-  auto load = [&](const uint8_t* base, int64_t at, int64_t st, const int (&off)[kDma], u32x4 (&codes)[kCodes], int tile,
-                  uint32_t plane) {
+  auto load = [&](auto is_v, const uint8_t* base, int64_t at, int64_t st, const int (&off)[kOffs],
+                  u32x4 (&codes)[kCodes], int tile, uint32_t plane) {
+    const int piece = tile * T::kPieces + wave;
+    const int from = (piece - win_base) & 63;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, from);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)at >> 32), from);
+    const auto rs = make_rsrc(base + (int64_t)(((uint64_t)hi << 32) | lo),
+                              16 * piece < p.tokens ? 15 * (int)st + (kFp8 ? D : 2 * D) : 0);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int hp = wave + i * kWaves;  // piece of the tile
-      const int piece = tile * T::kHalves + hp;
-      const int from = (piece - win_base) & 63;
-      const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, from);
-      const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)at >> 32), from);
-      const auto rs = make_rsrc(base + (int64_t)(((uint64_t)hi << 32) | lo),
-                                16 * piece < p.tokens ? 15 * (int)st + (kFp8 ? D : 2 * D) : 0);
-#pragma unroll
-      for (int r = 0; r < (kFp8 ? kCodeLoads : kDma); ++r) {
-        if constexpr (!kFp8) {
-          lds_dma16(rs, plane + hp * 16 * T::kRow + r * 1024, off[r]);
-        } else {
-          const int R = r * (1024 / D) + lane * 16 / D, d0 = lane * 16 % D;
-          const auto x = buf_load<16>(rs, R * (int)st + d0);
-          codes[i * kCodeLoads + r] = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
-        }
+    for (int r = 0; r < (kFp8 ? kCodeLoads : kDma); ++r) {
+      if constexpr (!kFp8) {
+        lds_dma16(rs, plane + wave * 16 * T::kRow + r * 1024, D <= 128 ? off[r % kOffs] : dma_off(is_v, r));
+      } else {
+        const int R = r * (1024 / D) + lane * 16 / D, d0 = lane * 16 % D;
+        const auto x = buf_load<16>(rs, R * (int)st + d0);
+        codes[r] = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
       }
     }
   };
@@ -204,39 +209,37 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
     if constexpr (kFp8) {
       constexpr bool kV = decltype(is_v)::value;
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i)
+      for (int r = 0; r < kCodeLoads; ++r) {
+        const int R = r * (1024 / D) + lane * 16 / D, m = lane * 16 % D / 8;
+        const int swz = kV ? v_swizzle<T::kChunks>(R) : k_swizzle<T::kChunks>(R);
+        const u32x4 x = codes[r];
+        const uint32_t at = plane + (wave * 16 + R) * T::kRow;
 #pragma unroll
-        for (int r = 0; r < kCodeLoads; ++r) {
-          const int R = r * (1024 / D) + lane * 16 / D, m = lane * 16 % D / 8;
-          const int swz = kV ? v_swizzle<T::kChunks>(R) : k_swizzle<T::kChunks>(R);
-          const u32x4 x = codes[i * kCodeLoads + r];
-          const uint32_t at = plane + ((wave + i * kWaves) * 16 + R) * T::kRow;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const u32x2 lo = e4m3x4_to<kV ? kVBf16 : kQBf16>(x[2 * e]), hi = e4m3x4_to<kV ? kVBf16 : kQBf16>(x[2 * e + 1]);
-            *(lds_u32x4_w*)(uintptr_t)(at + 16 * ((m + e) ^ swz)) = u32x4{lo[0], lo[1], hi[0], hi[1]};
-          }
+        for (int e = 0; e < 2; ++e) {
+          const u32x2 lo = e4m3x4_to<kV ? kVBf16 : kQBf16>(x[2 * e]), hi = e4m3x4_to<kV ? kVBf16 : kQBf16>(x[2 * e + 1]);
+          *(lds_u32x4_w*)(uintptr_t)(at + 16 * ((m + e) ^ swz)) = u32x4{lo[0], lo[1], hi[0], hi[1]};
         }
+      }
     }
   };
   // (the window moves on when K, which runs a tile ahead of V, leaves it; V's pieces
   // of the tile before are still in it: 64 pieces are 16 tiles, kept from the
   // tile before the one that moves it)
   auto window = [&](int tile) {
-    if ((tile + 1) * T::kHalves - win_base > 64) {
-      win_base = (tile - 1) * T::kHalves;
+    if ((tile + 1) * T::kPieces - win_base > 64) {
+      win_base = (tile - 1) * T::kPieces;
       place(page_of(win_base + lane));
     }
   };
   auto load_k = [&](int tile) {
     window(tile);
-    load(kbase, k_piece, p.k_st, k_off, k_codes, tile, lds + ((tile - tile0) & 1) * T::kPlane);
+    if (T::kSplit == 1 || part == 0) load(std::false_type{}, kbase, k_piece, p.k_st, k_off, k_codes, tile, lds + ((tile - tile0) & 1) * T::kPlane);
   };
   auto load_v = [&](int tile) {
-    load(vbase, v_piece, p.v_st, v_off, v_codes, tile, lds + (2 + ((tile - tile0) & 1)) * T::kPlane);
+    if (T::kSplit == 1 || part == 1) load(std::true_type{}, vbase, v_piece, p.v_st, v_off, v_codes, tile, lds + (2 + ((tile - tile0) & 1)) * T::kPlane);
   };
-  auto put_k = [&](int tile) { put(std::false_type{}, k_codes, lds + ((tile - tile0) & 1) * T::kPlane); };
-  auto put_v = [&](int tile) { put(std::true_type{}, v_codes, lds + (2 + ((tile - tile0) & 1)) * T::kPlane); };
+  auto put_k = [&](int tile) { if (T::kSplit == 1 || part == 0) put(std::false_type{}, k_codes, lds + ((tile - tile0) & 1) * T::kPlane); };
+  auto put_v = [&](int tile) { if (T::kSplit == 1 || part == 1) put(std::true_type{}, v_codes, lds + (2 + ((tile - tile0) & 1)) * T::kPlane); };
   load_k(tile0);
   load_v(tile0);
 
@@ -245,8 +248,8 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
   // at all of them: the waves take one path, which holds barriers).
   const int first = tile0 * T::kTile, end = min(tile1 * T::kTile, p.tokens);  // the chunk's tokens
   bool ends_inside = false;
-  for (int r = lane; r < 32 * kWaves; r += kWave) {
-    const int rr = min(rt * 32 * kWaves + r, p.rows - 1);
+  for (int r = lane; r < kRows; r += kWave) {
+    const int rr = min(rt * kRows + r, p.rows - 1);
     const int l = p.lens[fdiv((uint32_t)rr, p.g_div)];
     ends_inside = ends_inside || (l > first && l < end);
   }
@@ -266,18 +269,23 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
 
   // ---- operand addresses: the chunk of a k-step (dim block) is an XOR away, tile
   // row and buffer a constant offset
-  uint32_t k_at[kSteps], v_at[kDb];
+  constexpr int kKeep = D <= 128 ? kSteps : 1;  // (head_dim 256: worked out where they are used)
+  uint32_t k_at[kKeep], v_at[kDb];
   {
     const int vj = lane & 15, vr = 4 * h + vj / 4;
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i)
+    for (int i = 0; i < kKeep; ++i)
       k_at[i] = lds + ((c * T::kRow + 16 * (h ^ k_swizzle<T::kChunks>(c))) ^ (32 * i));
 #pragma unroll
     for (int d = 0; d < kDb; ++d)
       v_at[d] = lds + 2 * T::kPlane + ((vr * T::kRow + 16 * ((2 * (c >> 4) + (vj & 3) / 2) ^ v_swizzle<T::kChunks>(vr)) +
-                                    8 * (vj & 1)) ^ (64 * d));
+                                    8 * (vj & 1)) ^ (64 * (part * kDb + d)));
   }
-  auto k_operand = [&](uint32_t off, int i) { return *(lds_u32x4*)((lds_u8*)(uintptr_t)k_at[i] + off); };
+  // (at head_dim 256 the tile starts at a multiple of 512 past `lds`: the XOR stays within its row)
+  auto k_operand = [&](uint32_t off, int i) {
+    const uint32_t at = kKeep == kSteps ? k_at[i % kKeep] : lds + ((k_at[0] - lds) ^ (32 * i));
+    return *(lds_u32x4*)((lds_u8*)(uintptr_t)at + off);
+  };
   auto v_operand = [&](uint32_t off, int st, int d) {
     const u32x2 lo = lds_read_tr16(v_at[d] + (off + st * 16 * T::kRow));
     const u32x2 hi = lds_read_tr16(v_at[d] + (off + st * 16 * T::kRow + 8 * T::kRow));
@@ -286,7 +294,7 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
 
   auto turn_k = [&](int by) {
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) k_at[i] += by;
+    for (int i = 0; i < kKeep; ++i) k_at[i] += by;
   };
   auto turn_v = [&](int by) {
 #pragma unroll
@@ -385,10 +393,10 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
   auto stage = [&](auto qk, auto pv, uint32_t k_blk, uint32_t v_blk, f32x16& s_next, const f32x16& s,
                    const Weights& w_prev, float& m) {
     constexpr bool kQk = decltype(qk)::value, kPv = decltype(pv)::value;
-    static_assert(kSteps == 2 * kDb, "a k-step of QK for every V operand");
-    constexpr int kPer = (kQk ? 1 : 0) + (kPv ? (kVBf16 ? 2 : 1) : 0);
-    constexpr int kSlots = kSteps * kPer, kTimes = 13, kAhead = 2;
-    u32x4 kop[kSteps], vop[kSteps];
+    constexpr int kVs = 2 * kDb, kRatio = kSteps / kVs;  // V operands, and QK k-steps for each
+    constexpr int kPer = kVBf16 ? 2 : 1;                  // matrix instructions of a V operand
+    constexpr int kSlots = (kQk ? kSteps : 0) + (kPv ? kVs * kPer : 0), kTimes = 13, kAhead = 2;
+    u32x4 kop[kSteps], vop[kVs];
     float x[16], mt = -INFINITY, m_use = 0.f;
     Weights w;
     w.sum = 0.f;
@@ -431,7 +439,14 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
     auto read = [&](int i) {
       if (i >= kSteps) return;
       if constexpr (kQk) kop[i] = k_operand(k_blk, i);
-      if constexpr (kPv) vop[i] = v_operand(v_blk, i / kDb, i % kDb);
+      if (kPv && i % kRatio == 0) vop[i / kRatio] = v_operand(v_blk, i / kRatio / kDb, i / kRatio % kDb);
+    };
+    int n = 0;
+    auto rest = [&]() {  // of slot n
+#pragma unroll
+      for (int t = n * kTimes / kSlots; t < (n + 1) * kTimes / kSlots; ++t) step(t);
+      ++n;
+      __builtin_amdgcn_sched_barrier(0);
     };
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -440,27 +455,40 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
 #pragma unroll
       for (int i = 0; i < 16; ++i) s_next[i] = 0.f;
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int n = 0; n < kSlots; ++n) {
-      const int i = n / kPer, which = n % kPer;
-      __builtin_amdgcn_sched_barrier(0);
-      if (kQk && which == 0) s_next = mfma32x32x16<kQBf16>(kop[i], qop[i], s_next);
-      if constexpr (kPv) {
-        if (which == kPer - (kVBf16 ? 2 : 1)) acc[i % kDb] = mfma32x32x16<kVBf16>(vop[i], w_prev.hi[i / kDb], acc[i % kDb]);
-        if (kVBf16 && which == kPer - 1) acc[i % kDb] = mfma32x32x16<true>(vop[i], w_prev.lo[i / kDb], acc[i % kDb]);
+    for (int i = 0; i < kSteps; ++i) {
+      if constexpr (kQk) {
+        s_next = mfma32x32x16<kQBf16>(kop[i], qop[i], s_next);
+        read(i + kAhead);
+        rest();
       }
-      if (which == 0) read(i + kAhead);
+      if (kPv && i % kRatio == kRatio - 1) {
+        const int j = i / kRatio;
+        acc[j % kDb] = mfma32x32x16<kVBf16>(vop[j], w_prev.hi[j / kDb], acc[j % kDb]);
+        if constexpr (!kQk) {
 #pragma unroll
-      for (int t = n * kTimes / kSlots; t < (n + 1) * kTimes / kSlots; ++t) step(t);
+          for (int k = 0; k < kRatio; ++k) read(i + 1 - kRatio + k + kAhead);
+        }
+        rest();
+        if constexpr (kVBf16) {
+          acc[j % kDb] = mfma32x32x16<true>(vop[j], w_prev.lo[j / kDb], acc[j % kDb]);
+          rest();
+        }
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
     return w;
   };
   // A tile whose tokens do not all count for every column (columns that end
-  // inside the prefix, the prefix's last tile).  V rows past a column's end may
-  // hold anything, and 0 x inf is NaN, so each block is multiplied once per
-  // different end, with V's rows zeroed past it, and only the columns of that
-  // end take the sum.
+  // inside the chunk, the prefix's last tile).  V rows past a column's end may
+  // hold anything, and 0 x inf is NaN, so from the wave's first end on each block
+  // is multiplied once per different end, with V's rows zeroed past it, and only
+  // the columns of that end take the sum.
+  int first_end = lim > first ? lim : p.tokens;  // (columns that end before the chunk are dropped at its end)
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) first_end = min(first_end, __shfl_xor(first_end, o));
+  first_end = uniform(first_end);
   auto compute_ends = [&](int tile) {
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb) {
@@ -474,6 +502,10 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
       const Weights w = weights(s, m_new);
       rescale(m_new);
       l_run += w.sum;
+      if (t0 + 32 <= first_end) {
+        values(off, w);
+        continue;
+      }
       uint64_t todo = __builtin_amdgcn_ballot_w64(lim > t0);
       while (todo) {
         const int last = __builtin_amdgcn_readlane(lim, __builtin_ctzll(todo));
@@ -566,16 +598,24 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
     }
     ++tile;
   }
+  if (tile < tile1 && tile > tile0) {  // (the first tile is loaded)
+    __syncthreads();
+    load_k(tile);
+    load_v(tile);
+    put_k(tile);
+    put_v(tile);
+  }
   for (; tile < tile1; ++tile) {
-    if (tile > tile0) {  // (the first tile is loaded)
-      __syncthreads();
-      load_k(tile);
-      load_v(tile);
-      put_k(tile);
-      put_v(tile);
-    }
     arrive();
+    if (tile + 1 < tile1) {
+      load_k(tile + 1);
+      load_v(tile + 1);
+    }
     if (live) compute_ends(tile);
+    if (tile + 1 < tile1) {
+      put_k(tile + 1);
+      put_v(tile + 1);
+    }
   }
 
   // ---- partials, relative to the maximum itself (the linear sink counts against it)
@@ -587,9 +627,9 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
   // stored like that, each instruction would touch 32 lines for 32 bytes each
   // (2.4 us of a 29 us kernel).  They go through LDS instead (piece m of row R at
   // m ^ R, so that neither side meets on a bank), a wave's rows in its own part.
-  constexpr int kPieceRow = D / 4;  // pieces of a row
+  constexpr int kPieceRow = D / T::kSplit / 4;  // pieces of the wave's part of a row
   __syncthreads();  // (every wave has done with K and V)
-  const uint32_t mine = lds + wave * (32 * D * 4);
+  const uint32_t mine = lds + wave_id * (32 * kPieceRow * 16);
 #pragma unroll
   for (int d = 0; d < kDb; ++d)
 #pragma unroll
@@ -601,31 +641,30 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
       *(lds_f32x4*)(uintptr_t)(mine + (c * kPieceRow + (m ^ (c & (kPieceRow - 1)))) * 16) = o;
     }
   const int64_t idx0 = ((int64_t)jc * p.Hkv + kvh) * p.rows + row0;  // the wave's first row
-  if (row_ok && h == 0) *(f32x2*)(p.part_ml + 2 * (idx0 + c)) = none ? f32x2{-INFINITY, 0.f} : f32x2{m_max, l_tot};
+  if (row_ok && h == 0 && part == 0) *(f32x2*)(p.part_ml + 2 * (idx0 + c)) = none ? f32x2{-INFINITY, 0.f} : f32x2{m_max, l_tot};
   const int n_pieces = min(32, p.rows - row0) * kPieceRow;  // (<= 0: a wave without rows)
-  float* dst = p.part_acc + idx0 * D;
+  float* dst = p.part_acc + idx0 * D + part * (D / T::kSplit);
 #pragma unroll
   for (int k = 0; k < kPieceRow / 2; ++k) {
     const int i = k * kWave + lane, R = i / kPieceRow, m = i % kPieceRow;
     const f32x4 o = *(lds_f32x4*)(uintptr_t)(mine + (R * kPieceRow + (m ^ (R & (kPieceRow - 1)))) * 16);
-    if (i < n_pieces) *(f32x4*)(dst + 4 * i) = o;
+    if (i < n_pieces) *(f32x4*)(dst + (int64_t)R * D + 4 * m) = o;
   }
 }
 
 // The whole of a shared decode but the merge: workgroups up to pp.blocks take the
 // prefix, the others the sequences' own tokens (partial_work, a wave each), so
 // that the own tokens' K and V stream in while the matrix cores are busy with
-// the prefix.  Registers and LDS let two workgroups on a CU; the first 256 of
-// each kind share the CUs.  In turn instead (prefix, own tokens, merge) 256 x
+// the prefix.  Registers and LDS let eight waves on a CU: two workgroups (the
+// first 256 of each kind share the CUs), at head_dim 256 one.  In turn instead (prefix, own tokens, merge) 256 x
 // 4096 + 128 tokens took 34 + 31 us in the first two.
 template <int D, int kKV>
 constexpr uint32_t shared_stage() {
-  constexpr uint32_t prefix = 4 * PrefixTile<D>::kPlane, own = kPrefixWaves * partial_stage<D, kKV>();
+  constexpr uint32_t prefix = 4 * PrefixTile<D>::kPlane, own = PrefixTile<D>::kWaves * partial_stage<D, kKV>();
   return prefix > own ? prefix : own;
 }
 template <int D, int kQ, int kKV>
-__global__ __launch_bounds__(64 * kPrefixWaves)
-    __attribute__((amdgpu_waves_per_eu(PrefixTile<D>::kPerEu, PrefixTile<D>::kPerEu)))
+__global__ __launch_bounds__(64 * PrefixTile<D>::kWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void shared_kernel(const int32_t* lens_arg, const int32_t* starts_arg, int B_arg, PrefixParams pp, Params pk) {
   extern __shared__ __attribute__((aligned(16))) uint8_t s_shared[];
   const uint32_t lds = (uint32_t)(uintptr_t)s_shared;
@@ -637,12 +676,12 @@ void shared_kernel(const int32_t* lens_arg, const int32_t* starts_arg, int B_arg
   p.lens = lens_arg;
   p.starts = starts_arg;
   p.B = B_arg;
-  // (wave w of workgroup b is worker w S + b of 4 S, S a multiple of 8: the
+  // (wave w of workgroup b is worker w S + b of kWaves S, S a multiple of 8: the
   // workers' numbers keep to the XCDs as those of one-wave workgroups do)
   const int b = (int)blockIdx.x - pp.blocks, S = (int)gridDim.x - pp.blocks;
   const int wave = uniform((int)threadIdx.x / kWave);
   partial_work<D, kQ, kKV, kPagedOwn, false, false, false>(
-      p, nullptr, Worker{(int)threadIdx.x & (kWave - 1), wave * S + b, kPrefixWaves * S},
+      p, nullptr, Worker{(int)threadIdx.x & (kWave - 1), wave * S + b, PrefixTile<D>::kWaves * S},
       lds + wave * partial_stage<D, kKV>(), (int32_t*)(s_shared + shared_stage<D, kKV>()) + wave * 2 * (p.B + 1));
 }
 
@@ -656,11 +695,13 @@ struct PrefixPlan {
 };
 PrefixPlan plan_prefix(int64_t rows, int Hkv, int D, int64_t tokens, int cus) {
   PrefixPlan pl;
-  pl.row_tiles = (int)cdiv(rows, 32 * kPrefixWaves);
+  pl.row_tiles = (int)cdiv(rows, 128);
   pl.tiles = (int)cdiv(tokens, 64);
-  // One workgroup a CU, two where each would have 24 tiles or more: with few tiles
-  // the partials' way to memory and back costs more than the second wave a SIMD gives.
-  const int64_t slots = (int64_t)cus * ((int64_t)pl.tiles * Hkv * pl.row_tiles >= 24 * (int64_t)cus && D <= 128 ? 2 : 1);
+  // One workgroup a CU, beside one of the own tokens': with two, the partials' way to
+  // memory and back (twice as many) costs as much as the second wave a SIMD gives,
+  // and the own tokens wait (us, with 0.5, 1, 2 a CU: 32 x 8192 bf16 39.5, 36.7, 47.4;
+  // 64 x 32768 e4m3 94.5, 61.2, 60.6; 256 x 4096 f16 59.9, 56.1, 68.7).
+  const int64_t slots = cus;
   const int64_t want = std::max<int64_t>(1, slots / ((int64_t)Hkv * pl.row_tiles));
   pl.chunk = (int)cdiv(pl.tiles, std::min<int64_t>(want, pl.tiles));
   pl.chunks = (int)cdiv(pl.tiles, pl.chunk);
@@ -668,9 +709,10 @@ PrefixPlan plan_prefix(int64_t rows, int Hkv, int D, int64_t tokens, int cus) {
 }
 // Sequences whose plan tables, one for each wave, fit LDS beside the tiles (160 KB
 // a CU, 128 KB of tiles at head_dim 256).
-constexpr int kSharedMaxBatch = 1000;
-constexpr uint32_t shared_tables(int B) { return kPrefixWaves * 8 * (uint32_t)(B + 1); }
-static_assert(shared_stage<256, kF16>() + shared_tables(kSharedMaxBatch) <= 160 * 1024, "tiles and tables fit LDS");
+constexpr int kSharedMaxBatch = 500;
+template <int D>
+constexpr uint32_t shared_tables(int B) { return PrefixTile<D>::kWaves * 8 * (uint32_t)(B + 1); }
+static_assert(shared_stage<256, kF16>() + shared_tables<256>(kSharedMaxBatch) <= 160 * 1024, "tiles and tables fit LDS");
 
 // The shared prefix of a decode (run_shared): the kernel's parameters and the
 // prefix partials that the reduce kernel takes in.
@@ -681,8 +723,8 @@ struct SharedPrefix {
 
 template <int D, int kQ, int kKV>
 void launch_shared_as(const SharedPrefix& sh, const Params& p, int own_blocks, const Launch& s) {
-  launch(shared_kernel<D, kQ, kKV>, dim3((unsigned)(sh.p.blocks + own_blocks)), dim3(64 * kPrefixWaves),
-         shared_stage<D, kKV>() + shared_tables(p.B), s, p.lens, p.starts, p.B, sh.p, p);
+  launch(shared_kernel<D, kQ, kKV>, dim3((unsigned)(sh.p.blocks + own_blocks)), dim3(64 * PrefixTile<D>::kWaves),
+         shared_stage<D, kKV>() + shared_tables<D>(p.B), s, p.lens, p.starts, p.B, sh.p, p);
 }
 template <int D>
 void launch_shared(const SharedPrefix& sh, const Params& p, int own_blocks, int q_dt, int kv_dt, const Launch& s) {

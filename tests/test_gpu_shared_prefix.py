@@ -13,12 +13,22 @@ import math
 import pytest
 import torch
 
-from fskernels.hip import decode as dec
+from fasterkernels_amd import native as nat
 from fskernels.hip import paged_flash_decode, paged_flash_decode_shared
 from fskernels.engine import DecodeGraph
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+
+
+@pytest.fixture(autouse=True)
+def always_shared():
+    """The small batches here on the shared kernels too."""
+    nat.set_option("share", 2)
+    yield
+    nat.set_option("share", 1)
+
+
 DT = {"f16": torch.float16, "bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}
 
 
@@ -273,6 +283,22 @@ def test_two_calls_at_once():
     torch.cuda.synchronize()
     for i, out in enumerate(got):
         assert torch.equal(out, (wa, wb)[i % 2])
+
+
+def test_which_calls_share():
+    """By the rule a small call is the paged decode's own, bit for bit, and a large one
+    is not; more sequences than the kernel takes are always the paged decode's."""
+    small = Batch([300 + i for i in range(4)], 256, (32, 8, 128), "f16", seed=21)
+    large = Batch([2100 + i for i in range(12)], 2048, (32, 8, 128), "f16", seed=22)
+    many = Batch([40 + i % 9 for i in range(501)], 32, (8, 1, 64), "f16", seed=23)
+    forced = small.run(), large.run()
+    assert torch.equal(many.run(), many.plain())
+    nat.set_option("share", 1)
+    assert torch.equal(small.run(), small.plain()) and not torch.equal(small.run(), forced[0])
+    assert torch.equal(large.run(), forced[1]) and not torch.equal(large.run(), large.plain())
+    check(large, large.run(), "large")
+    nat.set_option("share", 0)
+    assert torch.equal(large.run(), large.plain())
 
 
 def test_refusals():

@@ -42,7 +42,8 @@ def test_refusals(lib, override, code):
 def test_workspace(lib):
     f = lib.fsk_shared_workspace_bytes
     need = f(8, 32, 8, 128, 64, 16, 512)
-    assert lib.fsk_decode_paged_shared(*args(wsb=need - 1)) == nat.FSK_ERR_WORKSPACE
+    whole = lib.fsk_workspace_bytes(nat.FSK_LAYOUT_PAGED, 8, 32, 8, 128, 64, 16, 0)
+    assert need >= whole  # either way of decoding fits
     # less than a page shared: the paged decode's own workspace
     plain = lib.fsk_workspace_bytes(nat.FSK_LAYOUT_PAGED, 8, 32, 8, 128, 64, 16, 0)
     assert f(8, 32, 8, 128, 64, 16, 15) == plain
@@ -56,6 +57,13 @@ def test_workspace(lib):
         assert f(*a.values()) == getattr(nat, "FSK_ERR_" + code), bad
     # the largest batch and table: sizes stay positive
     assert f(16384, 1 << 16, 1, 256, (1 << 17) - 64, 16, 1 << 20) != 0
+
+
+def test_share_option(lib):
+    for bad in (-1, 3):
+        assert lib.fsk_set_option(b"share", bad) == nat.FSK_ERR_INVALID
+    for ok in (0, 2, 1):
+        assert lib.fsk_set_option(b"share", ok) == nat.FSK_OK
 
 
 def test_empty_batch_needs_no_gpu(lib):
