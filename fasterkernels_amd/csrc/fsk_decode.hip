@@ -469,9 +469,18 @@ __device__ __forceinline__ HalfTile half_tile(const Params& p, int b, int start,
   return h;
 }
 
-// A wave of the persistent grid: its lane, its number and how many there are.
-struct Worker {
-  int lane, id, count;
+// A wave of the persistent grid: its lane, its number and how many there are; as
+// a one-wave workgroup, or given.
+struct GridWorker {
+  __device__ __forceinline__ int lane() const { return threadIdx.x; }
+  __device__ __forceinline__ int id() const { return blockIdx.x; }
+  __device__ __forceinline__ int count() const { return gridDim.x; }
+};
+struct GivenWorker {
+  int lane_, id_, count_;
+  __device__ __forceinline__ int lane() const { return lane_; }
+  __device__ __forceinline__ int id() const { return id_; }
+  __device__ __forceinline__ int count() const { return count_; }
 };
 
 // Work plan.  The sequences' tokens are laid end to end, each sequence padded
@@ -659,11 +668,11 @@ __device__ __forceinline__ void seq_range_first(const Params& p, int lane, int& 
 
 // len0: length of sequence `lane` (0 past B), from seq_range_first, whose
 // loads the caller issues first.
-template <int kLayout, bool kScores>
+template <int kLayout, bool kScores, typename Worker>
 __device__ __forceinline__ Split build_plan(const Params& p, const Worker wk, int32_t* pre, int32_t* flat, const int len0,
                                             int& seg_out, int& flat0_out, int& pre0_out) {
   constexpr int kAlign = kScores ? 128 : 32;
-  const int lane = wk.lane;
+  const int lane = wk.lane();
   // Lengths of sequences lane, lane + 64, ...; the first block stays in a
   // register so that the common case (B <= 64) reads them once (and the
   // work loop reads them from these registers, not from memory).
@@ -750,7 +759,7 @@ __device__ __forceinline__ Split build_plan(const Params& p, const Worker wk, in
       pre0_out = pb;
     }
     if constexpr (kScores)
-      if (wk.id == 0 && b < p.B) p.lens_out[b] = len;
+      if (wk.id() == 0 && b < p.B) p.lens_out[b] = len;
     carry_f += __builtin_amdgcn_readlane(incl_f, kWave - 1);
     carry_u += __builtin_amdgcn_readlane(incl_u, kWave - 1);
   }
@@ -759,7 +768,7 @@ __device__ __forceinline__ Split build_plan(const Params& p, const Worker wk, in
     pre[p.B] = min(carry_u, p.u_max);
   }
   __syncthreads();
-  if (wk.id == 0) {
+  if (wk.id() == 0) {
     for (int b = lane; b <= p.B; b += kWave) p.plan[b] = pre[b];
   }
   return sp;
@@ -1339,7 +1348,7 @@ template <int D, int kKV>
 constexpr int partial_stage() {
   return ((D <= 128) ? FSK_PIPE_DEPTH : 1) * 2 * TileRegs<D, kKV>::kHalfBytes;
 }
-template <int D, int kQ, int kKV, int kLayout, bool kScores, bool kValu, bool kHostPlan>
+template <int D, int kQ, int kKV, int kLayout, bool kScores, bool kValu, bool kHostPlan, typename Worker>
 __device__ __forceinline__ void partial_work(const Params& p, const HostPlan* hp, const Worker wk,
                                              const uint32_t s_kstage, int32_t* s_plan) {
   using TR = TileRegs<D, kKV>;
@@ -1357,7 +1366,7 @@ __device__ __forceinline__ void partial_work(const Params& p, const HostPlan* hp
 
   int32_t* s_pre = s_plan;              // [B+1] first partial of each sequence
   int32_t* s_flat = s_plan + p.B + 1;   // [B+1] stream offset of each sequence
-  const int lane = wk.lane;
+  const int lane = wk.lane();
   const int g = lane >> 4;
   const int c = lane & 15;
 
@@ -1400,7 +1409,7 @@ __device__ __forceinline__ void partial_work(const Params& p, const HostPlan* hp
   if constexpr (kHostPlan) {
     // Workgroup 0 publishes the unit prefix for the reduce kernel, as
     // build_plan does (lanes past B hold pre[B]).
-    if (wk.id == 0) {
+    if (wk.id() == 0) {
       if (lane < p.B) p.plan[lane] = lane_pre;
       if (lane == 0) p.plan[p.B] = hp->pre_end;
     }
@@ -1431,7 +1440,7 @@ __device__ __forceinline__ void partial_work(const Params& p, const HostPlan* hp
   const bool pair = (kLayout == kVarlen && D == 128 && !kScores && !kValu) ? (uniform(p.pair) != 0) : false;
   const float sscale = p.score_scale * k_scale;
 
-  for (int w = wk.id; w < W; w += wk.count) {
+  for (int w = wk.id(); w < W; w += wk.count()) {
     int jc, hh;
     item_of(sp, (uint32_t)w, p.nh_div, jc, hh);
     const int kvh = (int)fdiv((uint32_t)hh, p.hb_div);  // (with pair: the pair index, n_hb = 1)
@@ -1671,8 +1680,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kWavesPerEu)
   extern __shared__ int32_t s_plan[];
   // LDS offset of the stage = low 32 bits of its generic address
   partial_work<D, kQ, kKV, kLayout, kScores, kValu, sizeof...(Plan) == 1>(
-      p, plan_ptr(host_plan...), Worker{(int)threadIdx.x, (int)blockIdx.x, (int)gridDim.x},
-      (uint32_t)(uintptr_t)s_kstage_mem, s_plan);
+      p, plan_ptr(host_plan...), GridWorker{}, (uint32_t)(uintptr_t)s_kstage_mem, s_plan);
 }
 
 // The sink folded into a row's denominator (M: the row's maximum score, log2

@@ -681,7 +681,7 @@ void shared_kernel(const int32_t* lens_arg, const int32_t* starts_arg, int B_arg
   const int b = (int)blockIdx.x - pp.blocks, S = (int)gridDim.x - pp.blocks;
   const int wave = uniform((int)threadIdx.x / kWave);
   partial_work<D, kQ, kKV, kPagedOwn, false, false, false>(
-      p, nullptr, Worker{(int)threadIdx.x & (kWave - 1), wave * S + b, PrefixTile<D>::kWaves * S},
+      p, nullptr, GivenWorker{(int)threadIdx.x & (kWave - 1), wave * S + b, PrefixTile<D>::kWaves * S},
       lds + wave * partial_stage<D, kKV>(), (int32_t*)(s_shared + shared_stage<D, kKV>()) + wave * 2 * (p.B + 1));
 }
 
