@@ -23,12 +23,13 @@ graph's memory pool at capture time.
 """
 from __future__ import annotations
 
-from typing import Callable, List, Optional, Sequence
+from typing import Callable, List, Optional, Sequence, Tuple
 
 import torch
 
-from ..hip.decode import paged_flash_decode
+from ..hip.decode import paged_flash_decode, paged_flash_decode_shared
 from ..hip.kv_write import paged_kv_write
+from ..hip.rotary import paged_kv_write_rope
 from ..paged_attn.paged_kv_cache import PAGE_SIZE, PagedKVCache
 
 
@@ -69,12 +70,22 @@ class PagedDecodeStep:
     for the batch inside the graph); slots and block-table stores (int64) and
     lengths (int32) reach the device in two small host-to-device copies per
     step.
+
+    ``rope=(cos, sin)`` (tables [positions, rotary_dim / 2]) takes queries and
+    keys as the projection gives them: the write normalises (``q_weight``,
+    ``k_weight``) and rotates them by each sequence's position on the way
+    (``paged_kv_write_rope``), still in two or three launches a step.
+    ``share_prefix=True`` attends the pages that all sequences share when the step
+    is captured (``cache.shared_prefix_len``) once for the batch; a step after one
+    of them was freed and its slot given to a sequence without those pages raises.
     """
 
     def __init__(self, cache: PagedKVCache, layer_idx: int, seq_ids: Sequence[int], num_q_heads: int, *,
                  q_dtype: Optional[torch.dtype] = None, src_dtype: Optional[torch.dtype] = None,
                  out_dtype: Optional[torch.dtype] = None, s_aux: Optional[torch.Tensor] = None,
-                 sink_mode: str = "linear"):
+                 sink_mode: str = "linear", rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 interleaved: bool = False, share_prefix: bool = False):
         cache._require_gpu()
         self.cache = cache
         self.layer = int(layer_idx)
@@ -91,22 +102,37 @@ class PagedDecodeStep:
         self.q = torch.zeros(B, num_q_heads, D, dtype=qdt, device=dev)
         self.k_new = torch.zeros(B, Hkv, D, dtype=sdt, device=dev)
         self.v_new = torch.zeros_like(self.k_new)
-        # device meta: slots [B] | block-table stores [B, 2] (int64), lengths [B] (int32)
-        self._meta = torch.full((3 * B,), -1, dtype=torch.int64, device=dev)
+        if rope is None and (q_weight is not None or k_weight is not None):
+            raise ValueError("q_weight and k_weight need rope=(cos, sin)")
+        # device meta: slots [B] | block-table stores [B, 2] | positions [B] (int64), lengths [B] (int32)
+        self._meta = torch.full((4 * B,), -1, dtype=torch.int64, device=dev)
         self._lens = torch.zeros(B, dtype=torch.int32, device=dev)
         self._rows = torch.tensor(self.seq_ids, dtype=torch.long, device=dev)
         slots = self._meta[:B]
-        upd = self._meta[B:].view(B, 2)
+        upd = self._meta[B:3 * B].view(B, 2)
+        positions = self._meta[3 * B:]
         bt = cache.block_table
         kp, vp = cache.k_pool[self.layer], cache.v_pool[self.layer]
         ks, vs = cache.k_scale, cache.v_scale
+        self.shared_len = cache.shared_prefix_len(self.seq_ids) if share_prefix else 0
+        self._frees = cache._frees
+        self._positions = rope[0].shape[0] if rope is not None else None
 
         def step_fn():
-            paged_kv_write(self.k_new, self.v_new, kp, vp, slots, k_scale=ks, v_scale=vs,
-                           block_table=bt, bt_updates=upd)
-            return paged_flash_decode(self.q, kp, vp, bt.index_select(0, self._rows), self._lens, PAGE_SIZE,
-                                      s_aux=s_aux, k_scale=ks, v_scale=vs, out_dtype=out_dtype,
-                                      sink_mode=sink_mode)
+            q = self.q
+            if rope is None:
+                paged_kv_write(self.k_new, self.v_new, kp, vp, slots, k_scale=ks, v_scale=vs,
+                               block_table=bt, bt_updates=upd)
+            else:
+                q = paged_kv_write_rope(q, self.k_new, self.v_new, kp, vp, slots, *rope, positions,
+                                        q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved,
+                                        k_scale=ks, v_scale=vs, block_table=bt, bt_updates=upd)
+            table = bt.index_select(0, self._rows)
+            if self.shared_len:
+                return paged_flash_decode_shared(q, kp, vp, table, self._lens, PAGE_SIZE, self.shared_len, s_aux=s_aux,
+                                                 k_scale=ks, v_scale=vs, out_dtype=out_dtype, sink_mode=sink_mode)
+            return paged_flash_decode(q, kp, vp, table, self._lens, PAGE_SIZE, s_aux=s_aux, k_scale=ks, v_scale=vs,
+                                      out_dtype=out_dtype, sink_mode=sink_mode)
 
         # capture with every token skipped and no table stores: nothing changes
         self._graph = DecodeGraph(step_fn, warmup=1)
@@ -122,8 +148,15 @@ class PagedDecodeStep:
         if v_new is not None:
             self.v_new.copy_(v_new.reshape(self.v_new.shape))
         B = len(self.seq_ids)
+        at = [self.cache._seq_lens[s] for s in self.seq_ids]  # the new tokens' positions
+        if self._positions is not None and max(at) >= self._positions:
+            raise IndexError(f"position {max(at)} is past the {self._positions} rows of rope's tables")
+        if self.shared_len and self._frees != self.cache._frees:
+            if self.cache.shared_prefix_len(self.seq_ids) < self.shared_len:
+                raise RuntimeError("the sequences no longer share the prefix that this step was captured with")
+            self._frees = self.cache._frees
         slots, updates = self.cache._plan(self.seq_ids, 1)
-        meta = slots + [-1] * (2 * B)
+        meta = slots + [-1] * (2 * B) + at
         for j, (flat, page) in enumerate(updates):
             meta[B + 2 * j] = flat
             meta[B + 2 * j + 1] = page

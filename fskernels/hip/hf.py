@@ -40,6 +40,7 @@ Differences from the reference, all deliberate:
 from __future__ import annotations
 
 import contextlib
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -48,6 +49,7 @@ from fasterkernels_amd import native as nat
 
 from .decode import (_on_gpu, _stream, decode_hf, decode_quantizing_to_fp8, flash_decode_gqa_hf_dense_optimized,
                      flash_decode_gqa_hf_fp8, quantize_each_to_fp8)
+from .rotary import qk_norm_rope
 
 _MASK_DTYPES = (torch.bool, torch.float16, torch.bfloat16, torch.float32)
 
@@ -204,3 +206,67 @@ def patched_hf_attention(fp8: bool = False, modeling_module=None):
         yield
     finally:
         modeling_module.eager_attention_forward = prev
+
+
+# ---------------------------------------------------------------------------
+# rotation of queries and keys
+# ---------------------------------------------------------------------------
+def _kernel_rotates(q, k, cos, sin) -> bool:
+    """Whether a rotary function's call is one that qk_norm_rope takes: 16-bit or
+    fp32 GPU tensors [B, H, S, D] with tables [B or 1, S, D] of whole heads, and
+    nothing that would have to be recorded."""
+    if any(type(t) is not torch.Tensor or not t.is_cuda for t in (q, k, cos, sin)):
+        return False
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, cos, sin)):
+        return False
+    if torch.compiler.is_compiling() or q.dim() != 4 or k.dim() != 4 or cos.dim() != 3 or sin.shape != cos.shape:
+        return False
+    B, _, S, D = q.shape
+    return (q.dtype in (torch.float16, torch.bfloat16, torch.float32) and k.dtype is q.dtype
+            and k.shape[0] == B and k.shape[2:] == q.shape[2:] and cos.shape[0] in (1, B) and cos.shape[1:] == (S, D)
+            and D % 16 == 0 and D <= 256 and cos.dtype in (torch.float16, torch.bfloat16, torch.float32)
+            and sin.dtype is cos.dtype and q.numel() > 0 and k.numel() > 0)
+
+
+def hf_rotary(original):
+    """``original`` (a model's ``apply_rotary_pos_emb(q, k, cos, sin,
+    unsqueeze_dim=1)``: q and k [B, H, S, D], tables [B or 1, S, D] whose two
+    halves are the same) on the rotation kernel, one launch in place of its
+    elementwise operations, in fp32 and rounded once.  Other calls, and those
+    that autograd records, go to ``original``."""
+
+    @functools.wraps(original)
+    def apply_rotary_pos_emb(q, k, cos, sin, *args, **kwargs):
+        plain = not args and kwargs.get("unsqueeze_dim", 1) == 1 and set(kwargs) <= {"unsqueeze_dim"}
+        if not plain or not _kernel_rotates(q, k, cos, sin):
+            return original(q, k, cos, sin, *args, **kwargs)
+        B, _, S, D = q.shape
+        rows = [t.transpose(1, 2).reshape(B * S, t.shape[1], D) for t in (q, k)]
+        tables = [t.reshape(-1, D)[:, :D // 2] for t in (cos, sin)]
+        return tuple(t.view(B, S, -1, D).transpose(1, 2) for t in qk_norm_rope(*rows, *tables))
+
+    apply_rotary_pos_emb._fsk_patch = True
+    return apply_rotary_pos_emb
+
+
+def patch_hf_rotary(modeling_module=None):
+    """Puts ``modeling_module.apply_rotary_pos_emb`` (default: transformers'
+    Qwen3 module) on the rotation kernel and returns the function it replaced."""
+    if modeling_module is None:
+        import transformers.models.qwen3.modeling_qwen3 as modeling_module
+    prev = modeling_module.apply_rotary_pos_emb
+    if not getattr(prev, "_fsk_patch", False):
+        modeling_module.apply_rotary_pos_emb = hf_rotary(prev)
+    return prev
+
+
+@contextlib.contextmanager
+def patched_hf_rotary(modeling_module=None):
+    """Context manager form of patch_hf_rotary; restores the previous function."""
+    if modeling_module is None:
+        import transformers.models.qwen3.modeling_qwen3 as modeling_module
+    prev = patch_hf_rotary(modeling_module)
+    try:
+        yield
+    finally:
+        modeling_module.apply_rotary_pos_emb = prev

@@ -33,6 +33,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 
 from ..hip.kv_write import paged_kv_write
+from ..hip.rotary import paged_kv_write_rope
 
 PAGE_SIZE = 16  # tokens per physical page
 
@@ -55,7 +56,13 @@ class PagedKVCache:
     Batched forms (no reference counterpart): ``append_kv_batch`` stores one
     token for each of several sequences in one launch; ``reserve_slots`` +
     ``write_kv`` take the slots of a step once and store every layer's rows
-    with one launch each.
+    with one launch each (``write_qkv_rope``: with the norms and the rotation of
+    queries and keys in the same launch).
+
+    Shared prompts (no reference counterpart): ``fork_sequence`` makes new
+    sequences that continue one's tokens in the same pages, and
+    ``shared_prefix_len`` says how many leading tokens of a batch lie in common
+    pages, which ``paged_flash_decode_shared`` attends once for the batch.
     """
 
     num_layers: int
@@ -82,6 +89,8 @@ class PagedKVCache:
         self._active: List[bool] = [False] * self.max_seqs
         self._free_pages: List[int] = list(range(self.num_pages))
         self._pages: List[List[int]] = [[] for _ in range(self.max_seqs)]
+        self._holders: List[int] = [0] * self.num_pages  # sequences that hold each page
+        self._frees = 0  # free_sequence calls: only they take tokens from a sequence
         self._journal = None  # (pages popped, {seq: (old length, old page count)}) of the call in progress
         if (self.k_scale is None) != (self.v_scale is None):
             raise ValueError("give both k_scale and v_scale or neither")
@@ -112,13 +121,17 @@ class PagedKVCache:
         raise RuntimeError("All sequence slots are occupied")
 
     def free_sequence(self, seq_id: int):
-        """Returns the sequence's pages to the free list in logical order (:93-101)."""
+        """Returns the sequence's pages, but those that a forked sequence still
+        holds, to the free list in logical order (:93-101)."""
+        self._frees += 1
         pages = self._pages[seq_id]
         n_pages = (self._seq_lens[seq_id] + PAGE_SIZE - 1) // PAGE_SIZE
         for lp in range(n_pages):
             pp = pages[lp] if lp < len(pages) else -1
             if pp >= 0:
-                self._free_pages.append(pp)
+                self._holders[pp] -= 1
+                if self._holders[pp] == 0:
+                    self._free_pages.append(pp)
         if n_pages:
             self.block_table[seq_id, :n_pages] = -1
         self._pages[seq_id] = []
@@ -129,9 +142,70 @@ class PagedKVCache:
         if not self._free_pages:
             raise RuntimeError("Out of KV pages")
         pp = self._free_pages.pop()
+        self._holders[pp] = 1
         if self._journal is not None:
             self._journal[0].append(pp)
         return pp
+
+    # ------------------------------------------------------------------
+    def fork_sequence(self, seq_id: int, n: int = 1) -> List[int]:
+        """``n`` new sequences that continue ``seq_id``'s tokens (samples of one
+        prompt, questions about one document): its full pages are shared, and a
+        page that it has begun is copied for each of them, so that every sequence
+        appends to pages of its own.  A shared page returns to the free list with
+        its last holder.  All or nothing: raises RuntimeError where slots or
+        pages do not suffice, before any state changes."""
+        n = int(n)
+        if not 0 <= seq_id < self.max_seqs or not self._active[seq_id]:
+            raise ValueError(f"sequence {seq_id} is not allocated")
+        if n < 0:
+            raise ValueError("n must not be negative")
+        length = self._seq_lens[seq_id]
+        full, rest = divmod(length, PAGE_SIZE)
+        if sum(not a for a in self._active) < n:
+            raise RuntimeError("All sequence slots are occupied")
+        if rest and len(self._free_pages) < n:
+            raise RuntimeError("Out of KV pages")
+        if n == 0:
+            return []
+        common = self._pages[seq_id][:full]
+        with self._all_or_nothing():  # (its body's device work comes before the slots are taken)
+            begun = [self._alloc_page() for _ in range(n)] if rest else []
+            ids = [sid for sid in range(self.max_seqs) if not self._active[sid]][:n]
+            if begun:
+                old = self._pages[seq_id][full]
+                at = torch.tensor(begun, dtype=torch.long, device=self.k_pool.device)
+                for pool in (self.k_pool, self.v_pool):
+                    # (as bytes: indexed stores of 8-bit floats)
+                    raw = pool.view(torch.uint8) if pool.element_size() == 1 else pool
+                    raw[:, at] = raw[:, old].unsqueeze(1)
+            if length:
+                rows = torch.tensor([common + begun[i:i + 1] for i in range(n)], dtype=torch.int32,
+                                    device=self.block_table.device)
+                self.block_table[torch.tensor(ids, device=self.block_table.device), :rows.shape[1]] = rows
+        for i, sid in enumerate(ids):
+            self._active[sid] = True
+            self._seq_lens[sid] = length
+            self._pages[sid] = common + begun[i:i + 1]
+            for pp in common:
+                self._holders[pp] += 1
+        return ids
+
+    def shared_prefix_len(self, seq_ids: Sequence[int]) -> int:
+        """Leading tokens of the listed sequences that lie in the same full pages
+        (a multiple of PAGE_SIZE): ``paged_flash_decode_shared``'s shared_len for
+        a batch of them.  It holds while none of them is
+        freed: sequences only grow."""
+        ids = list(seq_ids)
+        if not ids:
+            return 0
+        n = min(self._seq_lens[sid] for sid in ids) // PAGE_SIZE
+        first = self._pages[ids[0]]
+        for sid in ids[1:]:
+            pages = self._pages[sid]
+            if pages[:n] != first[:n]:
+                n = next(i for i in range(n) if pages[i] != first[i])
+        return n * PAGE_SIZE
 
     # ------------------------------------------------------------------
     def _plan(self, seq_ids: Sequence[int], num_tokens: int = 1) -> Tuple[List[int], List[Tuple[int, int]]]:
@@ -220,6 +294,8 @@ class PagedKVCache:
             for sid, (length, n_pages) in touched.items():
                 self._seq_lens[sid] = length
                 del self._pages[sid][n_pages:]
+            for pp in popped:
+                self._holders[pp] = 0
             self._free_pages.extend(reversed(popped))
             raise
         finally:
@@ -290,18 +366,29 @@ class PagedKVCache:
             slot_dev, upd_dev = self._stage(slots, updates)
             self._write(layer_idx, k, v, slot_dev, upd_dev)
 
-    def reserve_slots(self, seq_ids: Sequence[int], num_tokens: int = 1) -> torch.Tensor:
+    def reserve_slots(self, seq_ids: Sequence[int], num_tokens: int = 1, *, return_positions: bool = False):
         """Takes ``num_tokens`` new positions in each listed sequence (pages as
         needed, block table stored on the device) and returns their slots, an
         int64 device tensor [len(seq_ids) * num_tokens], sequence-major, for
-        ``write_kv`` of every layer (a host tensor for host pools)."""
+        ``write_kv`` of every layer (a host tensor for host pools).  With
+        ``return_positions``: ``(slots, positions)``, each token's place in its
+        sequence (int64, for ``write_qkv_rope``)."""
+        ids, n = list(seq_ids), int(num_tokens)
         with self._all_or_nothing():
-            slots, updates = self._plan(list(seq_ids), int(num_tokens))
-            slot_dev, upd_dev = self._stage(slots, updates)
+            positions = []
+            if return_positions:
+                lens = {}
+                for sid in ids:  # (a repeated id goes on where it stopped)
+                    at = lens.get(sid, self._seq_lens[sid])
+                    positions += range(at, at + n)
+                    lens[sid] = at + n
+            slots, updates = self._plan(ids, n)
+            both, upd_dev = self._stage(slots + positions, updates)  # (one copy for all three)
+            slot_dev, pos_dev = both[:len(slots)], both[len(slots):]
             if updates:
                 empty = self.k_pool.new_empty((0, self.num_kv_heads, self.head_dim), dtype=torch.float32)
                 self._write(0, empty, empty, slot_dev[:0], upd_dev)
-        return slot_dev
+        return (slot_dev, pos_dev) if return_positions else slot_dev
 
     def write_kv(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor):
         """Stores rows k/v ([n, Hkv, D], any strides with a contiguous head_dim,
@@ -314,6 +401,20 @@ class PagedKVCache:
             k = self._new_rows(k, "k", n)
             v = self._new_rows(v, "v", n)
             self._write_host(layer_idx, k, v, slot_mapping.to(self.k_pool.device))
+
+    def write_qkv_rope(self, layer_idx: int, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
+                       slot_mapping: torch.Tensor, positions: Optional[torch.Tensor], cos: torch.Tensor,
+                       sin: torch.Tensor, *, q_weight: Optional[torch.Tensor] = None,
+                       k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                       interleaved: bool = False) -> Optional[torch.Tensor]:
+        """``write_kv`` of one layer with the per-head norms and the rotation of
+        ``q`` and ``k`` in the same launch (``fskernels.hip.paged_kv_write_rope``):
+        stores the rotated keys and the values [n, Hkv, D] at slots from
+        ``reserve_slots`` and returns the rotated queries [n, Hq, D].  GPU pools only."""
+        self._require_gpu()
+        return paged_kv_write_rope(q, k, v, self.k_pool[layer_idx], self.v_pool[layer_idx], slot_mapping, cos, sin,
+                                   positions, q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved,
+                                   k_scale=self.k_scale, v_scale=self.v_scale)
 
     # ------------------------------------------------------------------
     def get_block_table_tensor(self, active_seq_ids: List[int]) -> torch.Tensor:
