@@ -18,6 +18,12 @@
 // DPP adds inside a 16-lane row.  A wave takes kRounds * 64 / T head rows of
 // one token, so its position, slot and table row are read once, with the first
 // rows' loads in flight.
+//
+// Bound by HBM at large sizes, by launch and two dependent round trips (position,
+// table row) at small ones.  Kernel times, bf16: 16384 tokens of 32 + 8 heads of 128
+// (344 MB) 59.5 us, 5.8 TB/s, above a plain copy's 4.9; into e4m3 pages 28001 tokens
+// with values (646 MB) 117 us, 5.5 TB/s; one token 3.4 us, of which an empty launch
+// is most.
 
 struct RopeParams {
   const uint8_t* src[3];                 // q, k, v rows [n, H, D]
@@ -398,7 +404,12 @@ int run_rope(const RopeArgs& a) {
   p.t_log = p.lanes <= 4 ? 2 : p.lanes <= 8 ? 3 : 4;
   p.interleaved = a.interleaved != 0;
   const uint32_t slots_per_wave = (uint32_t)kWave >> p.t_log;
-  const int rounds = a.n * cdiv(heads, slots_per_wave) >= 16 * (int64_t)device_cus() ? 2 : 1;
+  // A second round of rows per wave where one leaves more waves than the card holds
+  // at once (32 a CU), whose last ones would start late: bf16, 32 + 8 heads of 128 (us,
+  // 1 / 2 rounds): 64 tokens 3.6 / 4.0, 1024 5.3 / 5.6, 1600 6.9 / 7.5, 1700 8.7 / 7.4,
+  // 2048 9.3 / 7.9, 4096 16.8 / 17.0, 16384 60.6 / 57.5; into pages 1024 6.2 / 6.2,
+  // 1365 8.6 / 6.9, 2048 10.2 / 10.8.
+  const int rounds = a.n * cdiv(heads, slots_per_wave) > 28 * (int64_t)device_cus() ? 2 : 1;
   p.parts = (uint32_t)cdiv(heads, slots_per_wave * rounds);
   p.parts_div = make_fastdiv(p.parts);
   p.items = (uint32_t)(a.n * p.parts);
