@@ -71,7 +71,7 @@ class PagedDecodeStep:
     lengths (int32) reach the device in two small host-to-device copies per
     step.
 
-    ``rope=(cos, sin)`` (tables [positions, rotary_dim / 2]) takes queries and
+    ``rope=(cos, sin)`` (tables [positions, rotary_dim / 2], or None both) takes queries and
     keys as the projection gives them: the write normalises (``q_weight``,
     ``k_weight``) and rotates them by each sequence's position on the way
     (``paged_kv_write_rope``), still in two or three launches a step.
@@ -116,7 +116,8 @@ class PagedDecodeStep:
         ks, vs = cache.k_scale, cache.v_scale
         self.shared_len = cache.shared_prefix_len(self.seq_ids) if share_prefix else 0
         self._frees = cache._frees
-        self._positions = rope[0].shape[0] if rope is not None else None
+        tables = rope is not None and rope[0] is not None  # (None, None): norms only
+        self._positions = rope[0].shape[0] if tables else None
 
         def step_fn():
             q = self.q
@@ -124,7 +125,7 @@ class PagedDecodeStep:
                 paged_kv_write(self.k_new, self.v_new, kp, vp, slots, k_scale=ks, v_scale=vs,
                                block_table=bt, bt_updates=upd)
             else:
-                q = paged_kv_write_rope(q, self.k_new, self.v_new, kp, vp, slots, *rope, positions,
+                q = paged_kv_write_rope(q, self.k_new, self.v_new, kp, vp, slots, *rope, positions if tables else None,
                                         q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved,
                                         k_scale=ks, v_scale=vs, block_table=bt, bt_updates=upd)
             table = bt.index_select(0, self._rows)

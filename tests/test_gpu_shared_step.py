@@ -12,7 +12,7 @@ import torch
 from fasterkernels_amd import native as nat
 from fskernels.engine import PagedDecodeStep
 from fskernels.hip import hf as H
-from fskernels.hip import paged_flash_decode_shared
+from fskernels.hip import paged_flash_decode_shared, paged_kv_write_rope, qk_norm_rope
 from fskernels.paged_attn import PAGE_SIZE, PagedKVCache
 
 from .test_gpu_rope import DT, close, oracle, projection, table, weights
@@ -145,6 +145,11 @@ def test_captured_step_refuses_a_prefix_that_is_gone():
     with pytest.raises(RuntimeError, match="share"):
         step.step()
     assert cache._seq_lens == lens
+    normed = PagedDecodeStep(cache, 0, ids, 32, rope=(None, None), k_weight=torch.ones(128, device=DEV).half())
+    normed.step(k_new=torch.full((3, 8, 128), 2.0, device=DEV).half())
+    torch.cuda.synchronize()
+    page = cache._pages[ids[0]][(cache._seq_lens[ids[0]] - 1) // 16]
+    assert (cache.k_pool[0, page, :, (cache._seq_lens[ids[0]] - 1) % 16] == 1).all()  # 2 / sqrt(4 + 1e-6), rounded
     with pytest.raises(ValueError, match="rope"):
         PagedDecodeStep(cache, 0, ids, 32, q_weight=torch.ones(128, device=DEV))
 
@@ -231,3 +236,52 @@ def test_model_runs_through_the_rotary_patch():
     # fp32 throughout: the two differ by roundings of 2^-24 relative in the rotated rows,
     # which two layers of this width carry on (sums of at most 1024 products each)
     assert (got - want).abs().max() <= 1024 * 2.0 ** -24 * 16 * want.abs().max()
+
+
+# ---------------------------------------------------------------------------
+def table_of(rows, d):
+    return table(rows, d // 2, "f32", 13)
+
+
+def test_pools_past_four_gigabytes(share):
+    """Pages behind 2^32 bytes of a layer's pool, shared and own, written and read."""
+    P, hq, hkv, d, n = 140000, 32, 8, 128, 6
+    k_pool, v_pool = (torch.empty(P, hkv, 16, d, dtype=torch.float16, device=DEV) for _ in range(2))
+    assert k_pool.numel() * 2 > 1 << 32
+    g = torch.Generator().manual_seed(11)
+    prefix, lens = 256, [300 + 7 * i for i in range(n)]
+    shared = torch.cat([torch.arange(8), torch.arange(P - 8, P)])
+    own = torch.cat([torch.arange(8, 8 + 5 * n), torch.arange(P - 8 - 5 * n, P - 8)]).view(2, n, 5)
+    table = torch.cat([shared.expand(n, 16), own[1], own[0]], 1).int().to(DEV)
+    lens_t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    used = table.long().unique()
+    k_pool[used] = torch.randn(len(used), hkv, 16, d, generator=g).half().to(DEV)
+    v_pool[used] = torch.randn(len(used), hkv, 16, d, generator=g).half().to(DEV)
+    # the last token of every sequence through the writing rotation
+    q, k, v = projection(n, hq, hkv, d, "f16", 12)
+    cos, sin = table_of(400, d)
+    at = lens_t.long() - 1
+    slots = table.gather(1, (at // 16)[:, None]).long()[:, 0] * 16 + at % 16
+    assert (slots * hkv * d * 2 > 1 << 32).all()
+    qr = paged_kv_write_rope(q, k, v, k_pool, v_pool, slots, cos, sin, at)
+    close(k_pool[slots // 16, :, slots % 16], *oracle(k, None, cos, sin, at, 0, False), "f16", "keys")
+    assert torch.equal(v_pool[slots // 16, :, slots % 16], v)
+    out = paged_flash_decode_shared(qr, k_pool, v_pool, table, lens_t, 16, prefix)
+    b = Batch.__new__(Batch)
+    b.lens, b.heads, b.kv, b.page, b.table, b.q, b.k, b.v = lens, (hq, hkv, d), "f16", 16, table, qr, k_pool, v_pool
+    b.ks = b.vs = b.sinks = None
+    check(b, out, "far pages")
+
+
+def test_rows_past_four_gigabytes():
+    step = 1_200_000_000
+    base = torch.empty(2 * step + 8192, dtype=torch.bfloat16, device=DEV)
+    q = base.as_strided((3, 32, 128), (step, 128, 1))
+    k = base[4096:].as_strided((3, 8, 128), (step, 128, 1))
+    q.copy_(torch.randn(3, 32, 128, generator=torch.Generator().manual_seed(14)))
+    k.copy_(torch.randn(3, 8, 128, generator=torch.Generator().manual_seed(15)))
+    cos, sin = table_of(3, 128)
+    qo, ko = qk_norm_rope(q, k, cos, sin)
+    row = torch.arange(3)
+    close(qo, *oracle(q, None, cos, sin, row, 0, False), "bf16", "queries")
+    close(ko, *oracle(k, None, cos, sin, row, 0, False), "bf16", "keys")
