@@ -10,6 +10,18 @@
 // M-tile instead of once per sequence.  Softmax over shared and own tokens is
 // the log-sum-exp merge of the two parts, which the reduce kernel does with the
 // prefix's partials beside each sequence's own.
+//
+// Work: 4 M Hkv D flops a shared token against 2 Hkv D elements of K and V, so the
+// matrix cores bound long prefixes of wide batches and HBM the others.  Kernel /
+// whole call, us (the floor is the larger of the bytes at a copy's 4.9 TB/s and the
+// flops at a large product's 1.28 PF): 32 heads on 8 x 128, 32 sequences with 8192
+// shared bf16 tokens and 16 to 1024 own 28 / 34 (floor 18, bytes); 64 on 32768 e4m3
+// 57 / 62 (27, flops: 0.6 PF); 256 on 4096 f16 44 / 50 (33, bytes: 3.7 TB/s).  As
+// many single sequences (paged_flash_decode) these take 112, 601 and 303.  What a
+// prefix costs beyond its products is the serial part of each tile (barrier, first
+// operand reads, widening) and the ends of the kernel (work plan and first loads 4,
+// partials 6): without the softmax the second takes 56, with operands that are read
+// once 59, with K and V from the caches no less.
 
 struct PrefixParams {
   const uint8_t* q;
@@ -656,8 +668,9 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const uint32_
 // prefix, the others the sequences' own tokens (partial_work, a wave each), so
 // that the own tokens' K and V stream in while the matrix cores are busy with
 // the prefix.  Registers and LDS let eight waves on a CU: two workgroups (the
-// first 256 of each kind share the CUs), at head_dim 256 one.  In turn instead (prefix, own tokens, merge) 256 x
-// 4096 + 128 tokens took 34 + 31 us in the first two.
+// first 256 of each kind share the CUs), at head_dim 256 one.  In turn instead
+// (prefix, own tokens, merge) 256 x 4096 + 128 tokens took 34 + 31 us in the first
+// two, together they take 44.
 template <int D, int kKV>
 constexpr uint32_t shared_stage() {
   constexpr uint32_t prefix = 4 * PrefixTile<D>::kPlane, own = PrefixTile<D>::kWaves * partial_stage<D, kKV>();

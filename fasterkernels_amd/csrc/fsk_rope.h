@@ -405,11 +405,14 @@ int run_rope(const RopeArgs& a) {
   p.interleaved = a.interleaved != 0;
   const uint32_t slots_per_wave = (uint32_t)kWave >> p.t_log;
   // A second round of rows per wave where one leaves more waves than the card holds
-  // at once (32 a CU), whose last ones would start late: bf16, 32 + 8 heads of 128 (us,
-  // 1 / 2 rounds): 64 tokens 3.6 / 4.0, 1024 5.3 / 5.6, 1600 6.9 / 7.5, 1700 8.7 / 7.4,
-  // 2048 9.3 / 7.9, 4096 16.8 / 17.0, 16384 60.6 / 57.5; into pages 1024 6.2 / 6.2,
-  // 1365 8.6 / 6.9, 2048 10.2 / 10.8.
-  const int rounds = a.n * cdiv(heads, slots_per_wave) > 28 * (int64_t)device_cus() ? 2 : 1;
+  // at once (32 a CU), whose last ones would start late; for rows of four lanes, 16 to
+  // a wave, of which one round wastes more of a token's last wave, from half of that.
+  // Inputs from HBM, us, 1 / 2 rounds: bf16, 32 + 8 heads of 128: 64 tokens 3.3 / 3.7,
+  // 1024 5.9 / 6.4, 1400 (7000 waves) 7.3 / 8.0, 1700 9.5 / 8.5, 2048 10.5 / 9.5, 16384
+  // 64.5 / 60.7; into pages 820 6.1 / 6.4, 1365 9.6 / 8.0.  f16, 64 + 8 heads of 64: 600
+  // (3000 waves) 4.8 / 4.8, 820 5.6 / 5.5, 1237 7.7 / 6.9, 3000 14.7 / 14.7.
+  const int waves_a_cu = p.t_log == 2 ? 15 : 28;
+  const int rounds = a.n * cdiv(heads, slots_per_wave) > waves_a_cu * (int64_t)device_cus() ? 2 : 1;
   p.parts = (uint32_t)cdiv(heads, slots_per_wave * rounds);
   p.parts_div = make_fastdiv(p.parts);
   p.items = (uint32_t)(a.n * p.parts);
