@@ -24,9 +24,10 @@
 // A batch whose sequences share their first pages (fsk_prefix.h): shared_kernel
 // attends these once for all of them on the matrix cores, beside the partial
 // kernel's work on each sequence's own tokens, and shared_reduce_kernel merges both.
-// Around them: the norm and rotation of query and key rows (fsk_rope.h), the KV write, the e4m3 quantiser, the attended ranges of an HF
-// decode step, and the fp8 attention hook's decode, whose kernels (kinds kQuant
-// + type) quantise 16-bit K and V on the way to the matrix cores.
+// Around them: the norm and rotation of query and key rows (fsk_rope.h), the KV
+// write, the e4m3 quantiser, the attended ranges of an HF decode step, and the fp8
+// attention hook's decode, whose kernels (kinds kQuant + type) quantise 16-bit K
+// and V on the way to the matrix cores.
 //
 // The maths follows the reference kernels: scores s = q.k * sm_scale,
 // online softmax, P rounded to the KV compute type before P.V

@@ -1,6 +1,8 @@
 """The single HIP backend of the decode hot path (gfx950): it replaces the
 reference's fskernels.triton, fskernels.cuda and fskernels.tilelang decode
-modules.  The HF attention patches are in fskernels.hip.hf."""
+modules, and has operators beside them that the reference leaves to torch or lacks
+(the norm and rotation of queries and keys, the shared-prefix decode).  The HF
+attention and rotary patches are in fskernels.hip.hf."""
 from .decode import (FP8_DTYPE, FP8_MAX, flash_decode_gqa_hf_dense_optimized,
                      flash_decode_gqa_hf_fp8, flash_decode_gqa_varlen, fp8_decode_table,
                      paged_flash_decode, paged_flash_decode_shared, paged_gather, quantize_to_fp8, set_num_splits,
