@@ -22,8 +22,7 @@
 // Bound by HBM at large sizes, by launch and two dependent round trips (position,
 // table row) at small ones.  Kernel times, bf16: 16384 tokens of 32 + 8 heads of 128
 // (344 MB) 59.5 us, 5.8 TB/s, above a plain copy's 4.9; into e4m3 pages 28001 tokens
-// with values (646 MB) 117 us, 5.5 TB/s; one token 3.4 us, of which an empty launch
-// is most.
+// with values (646 MB) 117 us, 5.5 TB/s; one token 2.9 to 3.4 us.
 
 struct RopeParams {
   const uint8_t* src[3];                 // q, k, v rows [n, H, D]

@@ -29,8 +29,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor | None, sin
     ``k_weight`` [D]; None: y = x), then the pairs (t, t + R/2) of its first R
     dims, or (2t, 2t + 1) when ``interleaved``, turned by the angle of
     ``cos`` / ``sin`` [rows, R/2] at the token's row: (a cos - b sin, b cos +
-    a sin).  R is a multiple of 16; dims past it keep y.  Computed in fp32 and
-    rounded once.  ``positions`` (int64 or int32 [n]; values outside the table
+    a sin).  R is a multiple of 16; dims past it keep y.  Computed in fp32 (a row
+    whose sum of squares leaves its range, values past about 2^60, normalises to
+    zero) and rounded once.  ``positions`` (int64 or int32 [n]; values outside the table
     take its first or last row) gives each token's row; None: token i takes row
     i mod rows (tables made for these very tokens, or for one of several
     sequences of the same length).  ``cos = sin = None``: norms only.

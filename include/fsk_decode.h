@@ -344,7 +344,9 @@ FSK_API int fsk_paged_write(const void *k_new, int64_t k_stride_t, int64_t k_str
  *   y = x / sqrt(mean(x^2) + eps) * weight       (no norm where the weight is NULL)
  *   (y_i, y_j) = (y_i cos - y_j sin, y_j cos + y_i sin), cos = cos[p][t],
  * for t < rotary_dim / 2 and (i, j) = (t, t + rotary_dim / 2), or (2t, 2t + 1)
- * when `interleaved`; other dims keep y.  fp32 throughout, rounded once.
+ * when `interleaved`; other dims keep y.  fp32 throughout, rounded once (a row
+ * whose sum of squares leaves the fp32 range, values past about 2^60, normalises
+ * to zero).
  * cos / sin [table_rows, rotary_dim / 2] (row strides, 16-byte aligned rows) in
  * f16, bf16 or f32, shared by all heads; rotary_dim a multiple of 16 (0: norm
  * only, tables unused).  positions int64 [n] (device; values outside the table
