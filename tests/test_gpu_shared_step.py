@@ -285,3 +285,24 @@ def test_rows_past_four_gigabytes():
     row = torch.arange(3)
     close(qo, *oracle(q, None, cos, sin, row, 0, False), "bf16", "queries")
     close(ko, *oracle(k, None, cos, sin, row, 0, False), "bf16", "keys")
+
+
+@pytest.mark.parametrize("kv", ["f16", "e4m3"])
+def test_fork_in_a_cache_past_four_gigabytes(kv):
+    P = 140000 if kv == "f16" else 280000
+    cache = PagedKVCache(2, P, 8, 8, 8, 128, DT[kv], DEV)
+    assert cache.k_pool[0].numel() * cache.k_pool.element_size() > 1 << 32
+    a = cache.allocate_sequence()
+    g = torch.Generator().manual_seed(16)
+    slots = cache.reserve_slots([a], 21)
+    for layer in range(2):
+        cache.write_kv(layer, *(torch.randn(21, 8, 128, generator=g).to(DEV) for _ in range(2)), slots)
+    b, c = cache.fork_sequence(a, 2)
+    old, *new = [cache._pages[s][1] for s in (a, b, c)]
+    for pool in (cache.k_pool, cache.v_pool):
+        for layer in range(2):
+            want = pool[layer, old].float()
+            assert want[:, :5].any()
+            for page in new:
+                assert torch.equal(pool[layer, page].float(), want)
+        assert not pool[0, min(new) - 1].float().any()  # its neighbour is as it was
