@@ -3655,22 +3655,26 @@ SharedLayout shared_layout(const PrefixPlan& pl, int B, int Hq, int D) {
 int64_t shared_pages(int B, int64_t shared_len, int page_size) {
   return B == 0 || B > kSharedMaxBatch ? 0 : shared_len / page_size;
 }
-// Whether sharing pays: a call that the direct kernel would take is faster left to
-// it (32 heads on 8 x 128 fp16, 512 tokens shared by 8, 32, 64 sequences: 10.5,
-// 9.7, 12.1 us, shared 10.6, 13.4, 16.9), and the split kernels re-read a short
-// prefix from cache faster than the prefix's partials are merged, below 32 MB of
-// K/V re-reads (1024 tokens, 4, 8, 16, 64 sequences, 17 to 268 MB: 11.7, 13.2, 13.6,
-// 27.7 us, shared 11.9, 11.9, 13.2, 22.3; 64 heads on 8 x 64, 2048 tokens, 4, 8,
-// 32: 12.1, 13.8, 22.8, shared 11.1, 12.7, 16.8).  At head_dim 256, where one
-// workgroup fills a CU, below 64 MB, 256 MB for bf16 with its two products a weight
-// (fp16 4096 tokens, 4, 8, 16 sequences: 25.2, 38.0, 58.8, shared 28.0, 31.6, 35.7;
-// bf16 24.8, 38.4, 59.4, shared 36.0, 37.6, 41.5).
+// Whether sharing pays, by the bytes of K and V that it saves: those of the prefix for
+// every sequence but one.  The split kernels re-read them from cache, mostly, faster
+// than the prefix's partials are merged (us, as the paged decode / shared) below
+//   28 MB at head_dim 64 and 128 (fp16, 32 heads on 8 x 128: 2 x 4096 tokens 12.5 / 12.7,
+//   6 x 1024 11.9 / 11.5, 8 x 1024 12.5 / 11.9, 3 x 8192 16.1 / 14.7; e4m3 4 x 8192
+//   17.9 / 14.5; 64 heads on 8 x 64, 8 x 2048 13.8 / 12.7);
+//   at head_dim 256, where one workgroup fills a CU, 160 for fp16 (3 x 8192 33.8 / 35.3,
+//   6 x 4096 31.3 / 29.7, 8 x 4096 38.5 / 32.0), 250 for e4m3, widened on the way (12 x
+//   4096 34.4 / 37.5, 16 x 4096 42.2 / 39.4), and 280 for bf16 with two products a weight
+//   (3 x 16384 65.4 / 69.2, 5 x 9000 56.4 / 51.3, 10 x 4096 44.2 / 40.6).
+// The direct kernel, where it applies, is faster up to 300 MB (fp16, 128, 160 and 256 x
+// 512 tokens 23.1 / 25.7, 27.7 / 25.3, 42.1 / 31.7; e4m3, 128 and 192 x 768 24.3 / 24.4,
+// 32.0 / 26.5; bf16, 256 x 600 of 8 x 64 27.1 / 26.0), at head_dim 256 up to 600 (fp16,
+// 16 heads, 160 x 300, 377 MB, 39.7 / 39.5; bf16 216 x 230, 407 MB, 44.5 / 50.2).
 bool shared_pays(const Common& c, int64_t common) {
   if (g_opt.share != 1) return g_opt.share == 2;
-  if (direct_waves(c, (int64_t)c.B * plan_heads(c.layout, c.D, c.Hkv, c.Hq / c.Hkv), false)) return false;
-  const int64_t reads = c.B * common * c.page_size * 2 * c.Hkv * c.D * elem_bytes(c.kv_dt);
-  const int64_t least = c.D <= 128 ? 32 : c.kv_dt == FSK_BF16 ? 256 : 64;
-  return reads >= least * 1000000;
+  const double saved = (c.B - 1) * 2.0 * common * c.page_size * c.Hkv * c.D * elem_bytes(c.kv_dt);
+  int least = c.D <= 128 ? 28 : c.kv_dt == FSK_F16 ? 160 : c.kv_dt == FSK_E4M3 ? 250 : 280;
+  if (direct_waves(c, (int64_t)c.B * plan_heads(c.layout, c.D, c.Hkv, c.Hq / c.Hkv), false)) least = c.D <= 128 ? 300 : 600;
+  return saved >= least * 1e6;
 }
 int64_t shared_workspace(int B, int Hq, int Hkv, int D, int64_t max_blocks, int page_size, int64_t shared_len) {
   const int64_t whole = fsk_workspace_bytes(FSK_LAYOUT_PAGED, B, Hq, Hkv, D, max_blocks, page_size, 0);

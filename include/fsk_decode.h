@@ -508,8 +508,7 @@ FSK_API int fsk_decode_dense_fp8(const void *q, int64_t q_stride_b, int64_t q_st
  *                         split kernels.)
  *   "share"               shared-prefix decodes: 1 (default) the prefix is attended
  *                         once where that is faster than once per sequence (by the
- *                         K/V bytes that would be read again; not where the
- *                         direct kernel takes the whole call), 0 never, 2 always
+ *                         K/V bytes that would be read again), 0 never, 2 always
  *                         (up to 500 sequences in each case)
  *   "qk_engine"           0 (default): QK and PV on the matrix cores (MFMA);
  *                         1: the VALU formulation of the tile, for A/B
